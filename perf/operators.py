@@ -271,7 +271,7 @@ def _plain_append_one(x, codes, scale, page_of, slot, pages, old, code):
         lambda v: v.clamp(-top, top).to(CODES[code]))
     amax = torch.zeros_like(scale).index_reduce_(0, page_of, x.abs().amax(-1), "amax")
     was = torch.where(old[:, None], scale, torch.zeros_like(scale))
-    now = torch.maximum(was, (amax / top).clamp_min(SCALE_FLOOR))[pages]
+    now = torch.maximum(was, (amax / torch.full_like(amax, top)).clamp_min(SCALE_FLOOR))[pages]
     bits = codes.view(torch.uint8)
     earlier = bits[pages].view(codes.dtype).float()
     bits[pages] = cast(earlier * (was[pages] / now)[:, :, None, None]).view(torch.uint8)
