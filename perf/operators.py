@@ -341,7 +341,7 @@ def run(state):
         if case["op"] == "append":
             q = cache.append(state["k"], state["v"], state["lengths"], state["table"], offsets=state["offsets"],
                              q=state["q"], angles=state["angles"], layout=case["layout"])
-            k, v, k_scale, v_scale = cache.read(state["pages"], dtype=q.dtype)
+            k, v, k_scale, v_scale = cache.read(state["pages"], dtype=q.dtype, return_scales=True)
             return q, k, v, k_scale, v_scale
         return cache.attend(state["q"], state["lengths"], state["table"], offsets=state["offsets"],
                             max_new=state["most"], causal=case["causal"], window=case["window"] or None,
