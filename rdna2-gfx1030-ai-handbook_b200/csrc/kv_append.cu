@@ -1,0 +1,380 @@
+// Appends keys and values to a paged cache held in 8 bits, with the rotary
+// positions applied to the keys (and the call's queries) on the way.
+//
+// A page holds `page` tokens of a sequence for every kv head, K and V apart:
+// codes [page][dim] and one fp32 scale, so a token's value is code * scale.
+// For each (page, head) that receives tokens, with x the new tokens there
+// (keys after rotation), top = 127 or 448:
+//
+//   s   = max(s_old if the page holds earlier tokens, max|x| / top, 2^-100)
+//   c   = RNE(c * (s_old / s))            earlier codes, where s grew
+//   c   = clamp(RNE(x * fp32(1 / s)))     new codes
+//
+// A NaN or infinite token makes s NaN or infinite and with it the block.
+// Every division is IEEE, every product rounded on its own.
+#include "../../include/b2_attention.h"
+#include "b2_internal.h"
+#include "kv_common.cuh"
+
+namespace b2 {
+namespace {
+
+struct AppendParams {
+  Tokens tok;
+  const void* k;
+  const void* v;
+  int64_t k_token, k_head, v_token, v_head;
+  const int32_t* table;
+  int width;
+  uint8_t* k_codes;
+  uint8_t* v_codes;
+  float* k_scale;
+  float* v_scale;
+  int64_t pages;
+  int page, kv_heads;
+  const float* angles;
+  int64_t rows;
+  int rot, interleaved;
+  const void* q;
+  void* q_out;
+  int64_t q_token, q_head;
+  int q_heads;
+  int64_t slots;   // blocks of tokens this call may touch, at most
+  int64_t kv_ctas; // slots * kv_heads * 2, the rest of the grid rotates queries
+};
+
+constexpr int kAppendThreads = 256;
+
+// Slot s of the call belongs to the sequence with first_slot(b) <= s; the
+// slots of a sequence are enough for the blocks that its tokens touch,
+// floor((n - 2) / page) + 2 at most.
+__device__ __forceinline__ int64_t first_slot(const Tokens& tok, int b, int page) {
+  return static_cast<int64_t>(tok.begin(b)) / page + 2 * static_cast<int64_t>(b);
+}
+
+template <typename T, int DIM, int CODE>
+__device__ __forceinline__ void append_block(const AppendParams& p, int64_t item) {
+  constexpr int V = Vec<T>::kN;
+  constexpr int kLanes = DIM / (2 * V);  // lanes a token
+  constexpr int kRows = kAppendThreads / kLanes;
+  const bool is_v = item & 1;
+  const int head = static_cast<int>((item >> 1) % p.kv_heads);
+  const int64_t slot = (item >> 1) / p.kv_heads;
+
+  const int b = warp_search(p.tok.batch, slot, [&](int i) { return first_slot(p.tok, i, p.page); });
+  const int first = p.tok.begin(b);
+  const int count = p.tok.begin(b + 1) - first;
+  const int64_t start = static_cast<int64_t>(__ldg(p.tok.lengths + b)) - count;  // position of the first new token
+  // block index of this slot, and the positions [from, to) that it receives
+  const int64_t block = (start > 0 ? start : 0) / p.page + (slot - first_slot(p.tok, b, p.page));
+  int64_t from = block * p.page, to = from + p.page;
+  const bool earlier = from < start;
+  from = from > start ? from : start;
+  from = from > 0 ? from : 0;
+  to = to < start + count ? to : start + count;
+  if (from >= to || block >= p.width) return;
+  const int64_t page_id = __ldg(p.table + static_cast<int64_t>(b) * p.width + block);
+  if (page_id < 0 || page_id >= p.pages) return;
+
+  const int u = threadIdx.x % kLanes, row0 = threadIdx.x / kLanes;
+  const RotaryUnit unit = rotary_unit<V>(u, is_v ? 0 : p.rot, p.interleaved);
+  const T* x = static_cast<const T*>(is_v ? p.v : p.k) + head * (is_v ? p.v_head : p.k_head);
+  const int64_t x_token = is_v ? p.v_token : p.k_token;
+  uint8_t* codes = (is_v ? p.v_codes : p.k_codes) + (page_id * p.kv_heads + head) * p.page * DIM;
+  float* scale = (is_v ? p.v_scale : p.k_scale) + page_id * p.kv_heads + head;
+
+  const auto load = [&](int64_t position, float (&a)[V], float (&c)[V]) {
+    const T* row = x + (first + (position - start)) * x_token;
+    Vec<T>::unpack(ldg_v4(row + unit.o0), a);
+    Vec<T>::unpack(ldg_v4(row + unit.o1), c);
+    if (unit.pair >= 0) {
+      float cos[V], sin[V];
+      load_angles<V>(p.angles, p.rows, p.rot, position, unit.pair, cos, sin);
+      rotate_unit<V>(a, c, cos, sin, p.interleaved);
+    }
+  };
+
+  // largest magnitude as ordered bits: an infinity or a NaN stays on top
+  uint32_t top = 0;
+  for (int64_t pos = from + row0; pos < to; pos += kRows) {
+    float a[V], c[V];
+    load(pos, a, c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      top = max(top, __float_as_uint(a[i]) & 0x7fffffffu);
+      top = max(top, __float_as_uint(c[i]) & 0x7fffffffu);
+    }
+  }
+  __shared__ uint32_t tops[kAppendThreads / kWarp];
+  top = __reduce_max_sync(kFullMask, top);
+  if (threadIdx.x % kWarp == 0) tops[threadIdx.x / kWarp] = top;
+  const float was = earlier ? *scale : 0.0f;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kAppendThreads / kWarp; ++i) top = max(top, tops[i]);
+  float now = __fdiv_rn(__uint_as_float(top), CODE == kCodeInt8 ? 127.0f : 448.0f);
+  now = now < kScaleFloor ? kScaleFloor : now;
+  now = (was > now || was != was) ? was : now;
+
+  if (earlier && now != was) {
+    const float ratio = __fdiv_rn(was, now);
+    const int words = static_cast<int>(from - block * p.page) * (DIM / 4);
+    for (int i = threadIdx.x; i < words; i += kAppendThreads) {
+      const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[i];
+      uint32_t n = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        n |= to_code<CODE>(__fmul_rn(from_code<CODE>((w >> (8 * j)) & 0xffu), ratio)) << (8 * j);
+      reinterpret_cast<uint32_t*>(codes)[i] = n;
+    }
+  }
+  if (threadIdx.x == 0) *scale = now;
+
+  const float inv = __fdiv_rn(1.0f, now);
+  for (int64_t pos = from + row0; pos < to; pos += kRows) {
+    float a[V], c[V];
+    load(pos, a, c);
+    uint8_t* row = codes + (pos - block * p.page) * DIM;
+    uint32_t wa[V / 4], wc[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      wa[i] = wc[i] = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        wa[i] |= to_code<CODE>(__fmul_rn(a[4 * i + j], inv)) << (8 * j);
+        wc[i] |= to_code<CODE>(__fmul_rn(c[4 * i + j], inv)) << (8 * j);
+      }
+    }
+    if constexpr (V == 8) {
+      *reinterpret_cast<uint2*>(row + unit.o0) = make_uint2(wa[0], wa[1]);
+      *reinterpret_cast<uint2*>(row + unit.o1) = make_uint2(wc[0], wc[1]);
+    } else {
+      *reinterpret_cast<uint32_t*>(row + unit.o0) = wa[0];
+      *reinterpret_cast<uint32_t*>(row + unit.o1) = wc[0];
+    }
+  }
+}
+
+// Queries: a warp rotates 32 / lanes heads of one token, kQUnroll times.
+constexpr int kQUnroll = 4;
+
+template <typename T, int DIM>
+__device__ __forceinline__ void rotate_queries(const AppendParams& p, int64_t warp) {
+  constexpr int V = Vec<T>::kN;
+  constexpr int kLanes = DIM / (2 * V), kHeads = kWarp / kLanes;
+  const int chunks = (p.q_heads + kHeads * kQUnroll - 1) / (kHeads * kQUnroll);
+  const int64_t token = warp / chunks;
+  if (token >= p.tok.tokens) return;
+  const int b = p.tok.offsets == nullptr
+                    ? static_cast<int>(token) / p.tok.each
+                    : warp_search(p.tok.batch, token, [&](int i) { return static_cast<int64_t>(p.tok.begin(i)); });
+  const int64_t position = static_cast<int64_t>(__ldg(p.tok.lengths + b)) - p.tok.begin(b + 1) + token;
+  const int lane = threadIdx.x % kWarp;
+  const RotaryUnit unit = rotary_unit<V>(lane % kLanes, p.rot, p.interleaved);
+  float cos[V], sin[V];
+  if (unit.pair >= 0) load_angles<V>(p.angles, p.rows, p.rot, position, unit.pair, cos, sin);
+  const int head0 = static_cast<int>(warp % chunks) * kHeads * kQUnroll + lane / kLanes;
+  const T* x = static_cast<const T*>(p.q) + token * p.q_token;
+  T* out = static_cast<T*>(p.q_out) + token * p.q_heads * DIM;
+  uint4 va[kQUnroll], vb[kQUnroll];
+#pragma unroll
+  for (int i = 0; i < kQUnroll; ++i) {
+    const int h = head0 + i * kHeads;
+    if (h < p.q_heads) {
+      va[i] = ldg_v4(x + h * p.q_head + unit.o0);
+      vb[i] = ldg_v4(x + h * p.q_head + unit.o1);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kQUnroll; ++i) {
+    const int h = head0 + i * kHeads;
+    if (h < p.q_heads) {
+      if (unit.pair >= 0) {
+        float a[V], c[V];
+        Vec<T>::unpack(va[i], a);
+        Vec<T>::unpack(vb[i], c);
+        rotate_unit<V>(a, c, cos, sin, p.interleaved);
+        va[i] = Vec<T>::pack(a);
+        vb[i] = Vec<T>::pack(c);
+      }
+      *reinterpret_cast<uint4*>(out + h * DIM + unit.o0) = va[i];
+      *reinterpret_cast<uint4*>(out + h * DIM + unit.o1) = vb[i];
+    }
+  }
+}
+
+template <typename T, int DIM, int CODE>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendParams p) {
+  const int64_t cta = blockIdx.x;
+  if (cta < p.kv_ctas) {
+    append_block<T, DIM, CODE>(p, cta);
+  } else {
+    rotate_queries<T, DIM>(p, (cta - p.kv_ctas) * (kAppendThreads / kWarp) + threadIdx.x / kWarp);
+  }
+}
+
+template <typename T, int DIM, int CODE>
+cudaError_t run_append(AppendParams p, cudaStream_t stream) {
+  constexpr int kHeads = kWarp / (DIM / (2 * Vec<T>::kN));
+  p.slots = static_cast<int64_t>(p.tok.tokens) / p.page + 2 * static_cast<int64_t>(p.tok.batch);
+  p.kv_ctas = p.slots * p.kv_heads * 2;
+  const int64_t chunks = p.q != nullptr ? ceil_div64(p.q_heads, kHeads * kQUnroll) : 0;
+  const int64_t grid = p.kv_ctas + ceil_div64(chunks * p.tok.tokens, kAppendThreads / kWarp);
+  if (grid > INT32_MAX) return cudaErrorInvalidValue;
+  append_kernel<T, DIM, CODE><<<static_cast<unsigned>(grid), kAppendThreads, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T, int DIM>
+cudaError_t run_append_code(const AppendParams& p, int code, cudaStream_t s) {
+  return code == kCodeInt8 ? run_append<T, DIM, kCodeInt8>(p, s) : run_append<T, DIM, kCodeE4M3>(p, s);
+}
+
+template <typename T>
+cudaError_t run_append_dim(const AppendParams& p, int dim, int code, cudaStream_t s) {
+  return dim == 64 ? run_append_code<T, 64>(p, code, s) : run_append_code<T, 128>(p, code, s);
+}
+
+// ------------------------------------------------------------------ read back
+// Values of whole pages: [n][kv_heads][page][dim], K and V.
+template <typename T, int CODE>
+__global__ void __launch_bounds__(256) read_kernel(const uint8_t* k_codes, const uint8_t* v_codes, const float* k_scale,
+                                                   const float* v_scale, const int32_t* pages, int64_t n,
+                                                   int64_t num_pages, int kv_heads, int block_bytes, T* k_out, T* v_out,
+                                                   float* scales_out) {
+  const int64_t item = blockIdx.x;  // (page, head, K or V)
+  const bool is_v = item & 1;
+  const int head = static_cast<int>((item >> 1) % kv_heads);
+  const int64_t i = (item >> 1) / kv_heads;
+  const int64_t page = pages[i];
+  T* out = (is_v ? v_out : k_out) + (i * kv_heads + head) * block_bytes;
+  const bool held = page >= 0 && page < num_pages;
+  const float scale = held ? (is_v ? v_scale : k_scale)[page * kv_heads + head] : __int_as_float(0x7fffffff);
+  if (scales_out != nullptr && threadIdx.x == 0) scales_out[((is_v ? n : 0) + i) * kv_heads + head] = scale;
+  const uint8_t* codes = (is_v ? v_codes : k_codes) + (held ? (page * kv_heads + head) * block_bytes : 0);
+  for (int e = threadIdx.x * 8; e < block_bytes; e += 256 * 8) {
+    const uint2 w = held ? *reinterpret_cast<const uint2*>(codes + e) : make_uint2(0, 0);
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      f[j] = __fmul_rn(from_code<CODE>(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xffu), scale);
+#pragma unroll
+    for (int j = 0; j < 8; j += Vec<T>::kN) {
+      float part[Vec<T>::kN];
+#pragma unroll
+      for (int x = 0; x < Vec<T>::kN; ++x) part[x] = f[j + x];
+      *reinterpret_cast<uint4*>(out + e + j) = Vec<T>::pack(part);
+    }
+  }
+}
+
+template <typename T>
+cudaError_t run_read(const uint8_t* kc, const uint8_t* vc, const float* ks, const float* vs, const int32_t* pages,
+                     int64_t n, int64_t num_pages, int kv_heads, int block_bytes, int code, void* k_out, void* v_out,
+                     float* scales, cudaStream_t stream) {
+  const int64_t grid = n * kv_heads * 2;
+  if (grid > INT32_MAX) return cudaErrorInvalidValue;
+  const unsigned g = static_cast<unsigned>(grid);
+  if (code == kCodeInt8) {
+    read_kernel<T, kCodeInt8><<<g, 256, 0, stream>>>(kc, vc, ks, vs, pages, n, num_pages, kv_heads, block_bytes,
+                                                     static_cast<T*>(k_out), static_cast<T*>(v_out), scales);
+  } else {
+    read_kernel<T, kCodeE4M3><<<g, 256, 0, stream>>>(kc, vc, ks, vs, pages, n, num_pages, kv_heads, block_bytes,
+                                                     static_cast<T*>(k_out), static_cast<T*>(v_out), scales);
+  }
+  return cudaGetLastError();
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+}  // namespace
+}  // namespace b2
+
+extern "C" {
+
+int b2_kv_append(const void* k, const void* v, int dtype, int64_t tokens, int64_t kv_heads, int64_t dim,
+                 int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                 const int32_t* lengths, const int32_t* offsets, int64_t batch, const int32_t* table, int64_t width,
+                 const void* q, int64_t q_heads, int64_t q_token_stride, int64_t q_head_stride, void* q_out,
+                 const float* angles, int64_t angle_rows, int64_t rotary_dim, int layout, int code, void* k_codes,
+                 void* v_codes, float* k_scale, float* v_scale, int64_t pages, int64_t page, void* stream) {
+  const int invalid = static_cast<int>(cudaErrorInvalidValue);
+  if (dtype < b2::kF32 || dtype > b2::kBF16 || layout < 0 || layout > 1 || code < 0 || code > 1) return invalid;
+  if (tokens < 0 || tokens > INT32_MAX / 2 || batch < 0 || batch > (1 << 20) || width < 0 || width > INT32_MAX)
+    return invalid;
+  if (kv_heads < 1 || kv_heads > 65536 || (dim != 64 && dim != 128)) return invalid;
+  if (page != 16 && page != 32 && page != 64 && page != 128) return invalid;
+  if (pages < 0 || pages > INT32_MAX) return invalid;
+  if (tokens == 0) return 0;
+  if (batch < 1 || (offsets == nullptr && tokens % batch)) return invalid;
+  if (!k || !v || !lengths || (!table && width) || !k_codes || !v_codes || !k_scale || !v_scale) return invalid;
+  const int64_t unit = dtype == b2::kF32 ? 4 : 8;
+  const auto rows_ok = [&](const void* x, int64_t ts, int64_t hs) {
+    return b2::aligned16(x) && ts >= 0 && hs >= 0 && ts % unit == 0 && hs % unit == 0;
+  };
+  if (!rows_ok(k, k_token_stride, k_head_stride) || !rows_ok(v, v_token_stride, v_head_stride)) return invalid;
+  if (!b2::aligned16(k_codes) || !b2::aligned16(v_codes)) return invalid;
+  if (angles) {
+    if (!b2::aligned16(angles) || angle_rows < 1 || rotary_dim < 16 || rotary_dim % 16 || rotary_dim > dim)
+      return invalid;
+  }
+  if (q) {
+    if (q_heads < 1 || q_heads > 65536 || !angles || !q_out || !b2::aligned16(q_out)) return invalid;
+    if (!rows_ok(q, q_token_stride, q_head_stride)) return invalid;
+  }
+  b2::AppendParams p{};
+  p.tok = {lengths, offsets, static_cast<int>(batch), static_cast<int>(tokens), static_cast<int>(tokens / batch)};
+  p.k = k;
+  p.v = v;
+  p.k_token = k_token_stride;
+  p.k_head = k_head_stride;
+  p.v_token = v_token_stride;
+  p.v_head = v_head_stride;
+  p.table = table;
+  p.width = static_cast<int>(width);
+  p.k_codes = static_cast<uint8_t*>(k_codes);
+  p.v_codes = static_cast<uint8_t*>(v_codes);
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.pages = pages;
+  p.page = static_cast<int>(page);
+  p.kv_heads = static_cast<int>(kv_heads);
+  p.angles = angles;
+  p.rows = angle_rows;
+  p.rot = angles ? static_cast<int>(rotary_dim) : 0;
+  p.interleaved = layout == b2::kRotaryInterleaved;
+  p.q = q;
+  p.q_out = q_out;
+  p.q_token = q_token_stride;
+  p.q_head = q_head_stride;
+  p.q_heads = static_cast<int>(q_heads);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int d = static_cast<int>(dim);
+  if (dtype == b2::kF32) return static_cast<int>(b2::run_append_dim<float>(p, d, code, s));
+  if (dtype == b2::kF16) return static_cast<int>(b2::run_append_dim<__half>(p, d, code, s));
+  return static_cast<int>(b2::run_append_dim<__nv_bfloat16>(p, d, code, s));
+}
+
+int b2_kv_read(const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale, int code,
+               int64_t num_pages, int64_t kv_heads, int64_t page, int64_t dim, const int32_t* pages, int64_t n,
+               int dtype, void* k_out, void* v_out, float* scales_out, void* stream) {
+  const int invalid = static_cast<int>(cudaErrorInvalidValue);
+  if (code < 0 || code > 1 || dtype < b2::kF32 || dtype > b2::kBF16) return invalid;
+  if (num_pages < 0 || num_pages > INT32_MAX || kv_heads < 1 || kv_heads > 65536 || n < 0 || n > INT32_MAX)
+    return invalid;
+  if ((dim != 64 && dim != 128) || (page != 16 && page != 32 && page != 64 && page != 128)) return invalid;
+  if (n == 0) return 0;
+  if (!k_codes || !v_codes || !k_scale || !v_scale || !pages || !k_out || !v_out) return invalid;
+  if (!b2::aligned16(k_codes) || !b2::aligned16(v_codes) || !b2::aligned16(k_out) || !b2::aligned16(v_out))
+    return invalid;
+  const auto* kc = static_cast<const uint8_t*>(k_codes);
+  const auto* vc = static_cast<const uint8_t*>(v_codes);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int heads = static_cast<int>(kv_heads), bytes = static_cast<int>(page * dim);
+  const auto run = dtype == b2::kF32 ? b2::run_read<float> : dtype == b2::kF16 ? b2::run_read<__half>
+                                                                               : b2::run_read<__nv_bfloat16>;
+  return static_cast<int>(run(kc, vc, k_scale, v_scale, pages, n, num_pages, heads, bytes, code, k_out, v_out,
+                              scales_out, s));
+}
+
+}  // extern "C"

@@ -1,4 +1,4 @@
-"""ctypes binding of librdna2_b200.so (the sm_100a C ABI in include/b2_qlinear.h).
+"""ctypes binding of librdna2_b200.so (the sm_100a C ABI in include/*.h).
 
 Mirrors the reference's native-library loader (rdna2_ops/normalization.py:16-27):
 one cached CDLL, explicit argtypes, launches on torch's current stream.
@@ -26,7 +26,7 @@ DTYPE_CODE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torc
 
 _p, _i64, _int, _size = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
 
-# name -> (argtypes, restype); kept in step with include/b2_qlinear.h
+# name -> (argtypes, restype); kept in step with include/*.h
 SIGNATURES = {
     "b2_version": ([], _int),
     "b2_error_string": ([_int], ctypes.c_char_p),
@@ -82,6 +82,14 @@ SIGNATURES = {
                            _p], _int),
     "b2_shard_codes": ([_p, _int, _i64, _i64, _i64, _int, _int, _int, _int, _p, ctypes.POINTER(_p), _i64, _i64,
                         _p, ctypes.POINTER(_p), ctypes.c_uint32, _p], _int),
+    "b2_rotary": ([_p, _int, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _int, _int, _p, _int, _p, _i64, _i64, _p],
+                  _int),
+    "b2_kv_append": ([_p, _p, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _p, _i64, _p, _i64, _i64,
+                      _i64, _p, _p, _i64, _i64, _int, _int, _p, _p, _p, _p, _i64, _i64, _p], _int),
+    "b2_kv_read": ([_p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _p, _i64, _int, _p, _p, _p, _p], _int),
+    "b2_kv_attention_workspace_bytes": ([_i64] * 8, _size),
+    "b2_kv_attention": ([_p, _int, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _int, _p, _p, _p, _p, _i64,
+                         _i64, _i64, _i64, ctypes.c_float, _int, _i64, _p, _p, _p, _size, _p], _int),
     "b2_quant_linear_noalloc_max_bytes": ([], _size),
     "b2_quant_linear_noalloc": ([_int, _p, _int, _i64, _i64, _i64, _int, _p, _i64, _i64, _p, _i64,
                                  _p, _int, _int, _p, _int, _i64, _p], _int),
