@@ -1,0 +1,120 @@
+// What the two cached-attention kernels share: a call's parameters, which
+// cached tokens a row sees, and the arithmetic of the softmax.
+#pragma once
+
+#include "kv_common.cuh"
+
+namespace b2 {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct AttendParams {
+  Tokens tok;
+  const void* q;
+  int q_bf16;
+  int64_t q_token, q_head;
+  const int32_t* table;
+  int width;
+  const uint8_t* k_codes;
+  const uint8_t* v_codes;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t pages;
+  int page_shift, kv_heads, group;
+  float scale_log2;  // scale * log2(e)
+  int causal;
+  int64_t window;    // 0: none
+  void* out;
+  float* lse;
+  int* counters;     // [grid], zero between calls
+  float* partial;    // [grid][2] slots
+};
+
+// One sequence of the call.
+struct Sequence {
+  int first, count;     // rows of the call
+  int64_t start;        // position of the first one
+  int lo, hi;           // cached tokens that any row may see: [lo, hi)
+};
+
+__device__ __forceinline__ Sequence load_sequence(const AttendParams& p, int b) {
+  Sequence s;
+  s.first = p.tok.begin(b);
+  s.count = max(0, p.tok.begin(b + 1) - s.first);
+  const int length = __ldg(p.tok.lengths + b);
+  s.start = static_cast<int64_t>(length) - s.count;
+  const int64_t held = static_cast<int64_t>(p.width) << p.page_shift;
+  s.hi = static_cast<int>(max(int64_t(0), min(static_cast<int64_t>(length), held)));
+  int64_t lo = p.window > 0 ? s.start - p.window + 1 : 0;
+  s.lo = static_cast<int>(min(max(lo, int64_t(0)), static_cast<int64_t>(s.hi)));
+  return s;
+}
+
+// Cached tokens [lo, hi) that the row at `position` sees.
+__device__ __forceinline__ void row_bounds(const AttendParams& p, const Sequence& s, int64_t position, int& lo,
+                                           int& hi) {
+  hi = p.causal ? static_cast<int>(min(max(position + 1, int64_t(0)), static_cast<int64_t>(s.hi))) : s.hi;
+  lo = p.window > 0 ? static_cast<int>(min(max(position - p.window + 1, int64_t(0)), static_cast<int64_t>(s.hi))) : 0;
+}
+
+// A row's power of two: q * factor is below 2 in magnitude (4 at the very top
+// of the range), and q = (q * factor) * gain.
+__device__ __forceinline__ void row_power(uint32_t top_bits, float& factor, float& gain) {
+  const uint32_t e = min(max(top_bits >> 23, 1u), 253u);
+  factor = __uint_as_float((254u - e) << 23);
+  gain = __uint_as_float(e << 23);
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A block that no token was appended to may hold any scale: one at or below
+// zero has no logarithm and reads as the smallest scale.  NaN stays NaN.
+__device__ __forceinline__ float value_scale(float s) { return s < kScaleFloor ? kScaleFloor : s; }
+
+// log2 of a block's value scale, raised where it is 2^-64 of the largest one
+// that this warp has met: such a block's codes add nothing to the output, but
+// its p_j must not underflow, since the sum l still counts them.
+__device__ __forceinline__ float value_exponent(float scale, float gain_log2, float& largest) {
+  float lv = __log2f(value_scale(scale)) + gain_log2;
+  largest = fmaxf(largest, lv < 256.0f ? lv : largest);  // an infinite scale is a matter of its own block
+  const float least = largest - 64.0f;
+  return lv < least ? least : lv;
+}
+
+// Two running sums are joined relative to the larger maximum; a side that has
+// seen nothing has m = -inf and weight 0.
+__device__ __forceinline__ float weight_of(float m, float top) {
+  return top == -INFINITY ? 0.0f : exp2_approx(m - top);
+}
+
+// Tiles of 128 cached tokens x 256 query rows on the 5th-generation tensor
+// cores (kv_tiles.cu): the workspace and the launch of a call with many rows.
+size_t tiles_workspace_bytes(int64_t tokens, int64_t batch, int64_t group, int64_t kv_heads, int dim, int64_t width,
+                             int page);
+cudaError_t run_tiles(const AttendParams& p, int dim, int code, void* workspace, cudaStream_t stream);
+
+}  // namespace b2

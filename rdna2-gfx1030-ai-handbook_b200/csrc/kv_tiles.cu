@@ -1,0 +1,648 @@
+// Attention over the paged 8-bit cache for calls with many query rows, on
+// tcgen05 (the arithmetic is stated in kv_attention.cu).
+//
+// A CTA takes 256 rows of one sequence and kv head -- its tokens times the
+// head's query heads -- as two row tiles of 128, and walks the cached tokens
+// they see in tiles of 128.  Roles:
+//
+//   warps 0-3, 4-7  softmax of row tile 0 and 1, a thread a row: scores come
+//                   from tensor memory, weights go back there as fp16 over
+//                   the scores' own columns
+//   warps 8-11      codes -> fp16 operands in shared memory (128-byte swizzle),
+//                   two tiles of K and V each; every operand serves both row
+//                   tiles, so a code is converted once for 256 rows
+//   warp 12         issues the products: S_t = Q_t K^T (both operands in
+//                   shared memory) and O_t += P_t V (P_t in tensor memory, V
+//                   as stored: its channels are the contiguous dimension)
+//
+// The two row tiles alternate on the tensor cores: while one is in its
+// softmax the other multiplies.  O_t stays in tensor memory and is rescaled
+// only when a row's maximum has grown by more than 2^8 since the last time:
+// weights up to 2^8 are fp16 numbers as good as those up to 1.
+#include "../../include/b2_attention.h"
+#include "b2_internal.h"
+#include "kv_attention.cuh"
+
+namespace b2 {
+namespace {
+
+constexpr int kTileRows = 128;              // rows of one product (UMMA M)
+constexpr int kCtaRows = 2 * kTileRows;
+constexpr int kTileTokens = 128;
+constexpr int kGroups = kTileTokens / 16;   // a group of 16 tokens is in one block, whatever the page
+constexpr int kSoftmaxWarps = 8, kConvertWarps = 4;
+constexpr int kConvertThreads = kConvertWarps * kWarp;
+constexpr int kTilesThreads = (kSoftmaxWarps + kConvertWarps + 1) * kWarp;
+constexpr float kRescaleLog2 = 8.0f;
+
+// One row tile of queries, or one tile of K or V: panels of 64 channels, 128
+// rows of 128 bytes each, 128-byte swizzle.
+constexpr int kPanel = 128 * 128;
+
+struct GroupInfo {
+  float ks, lv, iv;  // key scale, log2 of the value scale, 2^(top_lv - lv)
+};
+
+template <int DIM>
+struct TilesShared {
+  static constexpr int kTile = DIM / 64 * kPanel;
+  static constexpr int kOffQ = 0;                     // 2 row tiles
+  static constexpr int kOffK = kOffQ + 2 * kTile;     // 2 stages
+  static constexpr int kOffV = kOffK + 2 * kTile;     // 2 stages
+  static constexpr int kOffCtl = kOffV + 2 * kTile;
+};
+
+struct TilesControl {
+  uint64_t k_full[2], k_free[2], v_full[2], v_free[2];
+  uint64_t s_full[2], p_full[2], o_done[2], info_full[4], last;
+  GroupInfo info[4][kGroups];
+  float top_lv[4];
+  uint32_t present[4];  // bit g: group g lies on a page of the cache
+  uint32_t tmem;
+  int abort, drained;
+};
+
+template <int DIM>
+constexpr int kTilesBytes = TilesShared<DIM>::kOffCtl + static_cast<int>(sizeof(TilesControl)) + 1024;
+
+struct TilesParams {
+  AttendParams a;
+  int64_t slots;  // row blocks of all sequences, at most
+  int splits;     // parts of the cached tokens that a row block is split into
+  float* partial; // [slots][heads][splits][256][DIM] sums, then [..][3][256] m, n, l
+  int* status;
+};
+
+// Slot s of the call is a row block of the sequence with first_block(b) <= s.
+__device__ __forceinline__ int64_t first_block(const AttendParams& p, int b) {
+  return static_cast<int64_t>(p.tok.begin(b)) * p.group / kCtaRows + b;
+}
+
+// A row block and the token tiles that any of its rows sees.
+struct Block {
+  Sequence s;
+  int b;
+  int64_t row0, rows;   // its first row, and the rows of the sequence
+  int tile0, tiles;
+};
+
+__device__ __forceinline__ bool load_block(const AttendParams& p, int64_t slot, Block& k) {
+  k.b = warp_search(p.tok.batch, slot, [&](int i) { return first_block(p, i); });
+  k.s = load_sequence(p, k.b);
+  k.rows = static_cast<int64_t>(k.s.count) * p.group;
+  k.row0 = (slot - first_block(p, k.b)) * kCtaRows;
+  if (k.row0 >= k.rows) return false;
+  int lo, hi, unused;
+  const int64_t last = min(k.row0 + kCtaRows, k.rows) - 1;
+  row_bounds(p, k.s, k.s.start + k.row0 / p.group, lo, unused);
+  row_bounds(p, k.s, k.s.start + last / p.group, unused, hi);
+  k.tile0 = lo / kTileTokens;
+  k.tiles = max(0, (hi + kTileTokens - 1) / kTileTokens - k.tile0);
+  return true;
+}
+
+// Parts that a block's tiles are split into, and the tiles of one part.
+__device__ __forceinline__ int part_tiles(const TilesParams& p, int tiles) { return (tiles + p.splits - 1) / p.splits; }
+__device__ __forceinline__ int part_count(const TilesParams& p, int tiles) {
+  const int per = part_tiles(p, tiles);
+  return per ? (tiles + per - 1) / per : 1;
+}
+
+__device__ __forceinline__ int64_t output_row(const AttendParams& p, const Sequence& s, int head, int64_t r) {
+  return (s.first + r / p.group) * static_cast<int64_t>(p.kv_heads * p.group) + head * p.group + r % p.group;
+}
+
+__device__ __forceinline__ uint32_t swizzled(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
+
+// Descriptor of V as the K x N operand with N (channels) contiguous: panels
+// of 64 channels kPanel apart, groups of 8 tokens 1024 bytes apart.
+__device__ __forceinline__ uint64_t channels_desc(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(kPanel >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// Bits [lo, hi) of a word.
+__device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
+  lo = max(lo, 0);
+  hi = min(hi, 32);
+  if (lo >= hi) return 0u;
+  return (hi == 32 ? 0xffffffffu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
+}
+
+template <int DIM, int CODE>
+__global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams tp) {
+  using Shared = TilesShared<DIM>;
+  constexpr int kPanels = DIM / 64;
+  const AttendParams& p = tp.a;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  TilesControl& ctl = *reinterpret_cast<TilesControl*>(smem + Shared::kOffCtl);
+  const uint32_t base_u32 = smem_u32(smem);
+  const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+
+  // the heaviest blocks of a causal prompt, its last rows, come first
+  const int64_t unit = blockIdx.x;
+  const int split = static_cast<int>(unit % tp.splits);
+  const int head = static_cast<int>(unit / tp.splits % p.kv_heads);
+  const int64_t slot = tp.slots - 1 - unit / tp.splits / p.kv_heads;
+  Block blk;
+  if (!load_block(p, slot, blk)) return;
+  const int per = part_tiles(tp, blk.tiles), parts = part_count(tp, blk.tiles);
+  if (split >= parts) return;
+  const int first = split * per;
+  const int count = min(per, blk.tiles - first);
+  const int token0 = (blk.tile0 + first) * kTileTokens;
+
+  if (warp == 12) {
+    if (lane == 0) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&ctl.k_full[i], kConvertWarps);
+        mbar_init(&ctl.v_full[i], kConvertWarps);
+        mbar_init(&ctl.k_free[i], 1);
+        mbar_init(&ctl.v_free[i], 1);
+        mbar_init(&ctl.s_full[i], 1);
+        mbar_init(&ctl.p_full[i], 4);
+        mbar_init(&ctl.o_done[i], 1);
+      }
+      for (int i = 0; i < 4; ++i) mbar_init(&ctl.info_full[i], 1);
+      mbar_init(&ctl.last, 1);
+      ctl.abort = ctl.drained = 0;
+      fence_mbar_init();
+    }
+    __syncwarp();
+    tmem_alloc(&ctl.tmem, 512);
+    tmem_relinquish();
+  }
+
+  // ---- queries: a softmax thread brings its own row
+  float qs = 0.0f;
+  int lo = 0, hi = 0;
+  const int tile = warp / 4, row = threadIdx.x % kTileRows;
+  const int64_t r = blk.row0 + tile * kTileRows + row;
+  const bool valid = warp < kSoftmaxWarps && r < blk.rows;
+  if (warp < kSoftmaxWarps) {
+    uint4 v[DIM / 8];
+    uint32_t top = 0;
+    const uint16_t* src = static_cast<const uint16_t*>(p.q) + (blk.s.first + r / p.group) * p.q_token +
+                          (head * p.group + r % p.group) * p.q_head;
+#pragma unroll
+    for (int c = 0; c < DIM / 8; ++c) {
+      v[c] = valid ? ldg_v4(src + 8 * c) : make_uint4(0, 0, 0, 0);
+      float f[8];
+      if (p.q_bf16) {
+        Vec<__nv_bfloat16>::unpack(v[c], f);
+      } else {
+        Vec<__half>::unpack(v[c], f);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+    }
+    float factor, gain;
+    row_power(top, factor, gain);
+    qs = gain * p.scale_log2;
+    if (valid) row_bounds(p, blk.s, blk.s.start + r / p.group, lo, hi);
+    uint8_t* dst = smem + Shared::kOffQ + tile * Shared::kTile;
+#pragma unroll
+    for (int c = 0; c < DIM / 8; ++c) {
+      float f[8];
+      if (p.q_bf16) {
+        Vec<__nv_bfloat16>::unpack(v[c], f);
+      } else {
+        Vec<__half>::unpack(v[c], f);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] *= factor;
+      *reinterpret_cast<uint4*>(dst + c / 8 * kPanel + swizzled(row, c % 8)) = Vec<__half>::pack(f);
+    }
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl.tmem;
+  volatile int* abort_flag = &ctl.abort;
+  // called by a whole warp, which leaves with one answer
+  const auto wait = [&](uint64_t* bar, uint32_t parity, int site) -> bool {
+    return __all_sync(kFullMask, mbar_wait(bar, parity, abort_flag, site, tp.status));
+  };
+
+  if (warp == 12) {
+    // ------------------------------------------------------- products
+    constexpr uint32_t kIdescS = make_idesc<kKindF16>(kTileRows, kTileTokens);
+    constexpr uint32_t kIdescO = make_idesc<kKindF16>(kTileRows, DIM) | (1u << 16);  // V: N contiguous
+    const auto scores = [&](int t, int stage) {
+      if (elect_one()) {
+        const uint32_t q = base_u32 + Shared::kOffQ + t * Shared::kTile;
+        const uint32_t k = base_u32 + Shared::kOffK + stage * Shared::kTile;
+#pragma unroll
+        for (int x = 0; x < DIM / 16; ++x) {
+          const uint32_t off = x / 4 * kPanel + x % 4 * 32;
+          umma<kKindF16>(tmem + t * 128, sw128_desc(q + off), sw128_desc(k + off), kIdescS, x > 0);
+        }
+        umma_commit(&ctl.s_full[t]);
+      }
+      __syncwarp();
+    };
+    const auto output = [&](int t, int stage, bool add) {
+      if (elect_one()) {
+        const uint32_t v = base_u32 + Shared::kOffV + stage * Shared::kTile;
+#pragma unroll
+        for (int x = 0; x < kTileTokens / 16; ++x)
+          umma_ts_f16(tmem + 256 + t * 128, tmem + t * 128 + 8 * x, channels_desc(v + x * 2048), kIdescO, add || x > 0);
+        umma_commit(&ctl.o_done[t]);
+      }
+      __syncwarp();
+    };
+    const auto commit = [&](uint64_t* bar) {
+      if (elect_one()) umma_commit(bar);
+      __syncwarp();
+    };
+    bool ok = true;
+    if (count > 0) {
+      ok = wait(&ctl.k_full[0], 0, kSiteMma);
+      if (ok) {
+        tc_fence_after();
+        scores(0, 0);
+        scores(1, 0);
+        commit(&ctl.k_free[0]);
+      }
+    }
+    for (int i = 0; ok && i < count; ++i) {
+      const int stage = i & 1, next = stage ^ 1;
+      const uint32_t parity = (i >> 1) & 1, next_parity = ((i + 1) >> 1) & 1;
+      ok = wait(&ctl.v_full[stage], parity, kSiteMma);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (!ok || !(ok = wait(&ctl.p_full[t], i & 1, kSiteMma))) break;
+        tc_fence_after();
+        output(t, stage, i > 0);
+        if (t == 1) commit(&ctl.v_free[stage]);
+        if (i + 1 < count) {
+          // the weights lie where the next scores go: they have been read first
+          ok = (t == 1 || wait(&ctl.k_full[next], next_parity, kSiteMma)) && wait(&ctl.o_done[t], i & 1, kSiteMma);
+          if (!ok) break;
+          tc_fence_after();
+          scores(t, next);
+          if (t == 1) commit(&ctl.k_free[next]);
+        }
+      }
+    }
+    // nothing is in flight when tensor memory is given back, after a wait
+    // that gave up either
+    commit(&ctl.last);
+    mbar_wait(&ctl.last, 0, &ctl.drained, kSiteMma, tp.status);
+    __syncwarp();
+  } else if (warp >= kSoftmaxWarps) {
+    // ------------------------------------------------------- codes to fp16
+    constexpr int kLoads = DIM / 16;       // 16-byte pieces of a tile a thread takes
+    constexpr int kRowsEach = 4;
+    const int tid = threadIdx.x - kSoftmaxWarps * kWarp;
+    const int chunk = tid % 4;             // quarter-warps take two rows: no bank conflicts below
+    int64_t at[kRowsEach];                 // where this thread's rows begin in the codes, or -1
+    const int page_mask = (1 << p.page_shift) - 1;
+    const auto block_of = [&](int token) -> int64_t {
+      if (token >= blk.s.hi) return -1;
+      const int64_t page = __ldg(p.table + static_cast<int64_t>(blk.b) * p.width + (token >> p.page_shift));
+      return page >= 0 && page < p.pages ? page * p.kv_heads + head : -1;
+    };
+    const auto locate = [&](int i) {
+#pragma unroll
+      for (int j = 0; j < kRowsEach; ++j) {
+        const int token = token0 + i * kTileTokens + tid / 4 + 32 * j;
+        const int64_t block = block_of(token & ~15);
+        at[j] = block < 0 ? -1 : ((block << p.page_shift) + (token & page_mask)) * DIM;
+      }
+    };
+    const auto load = [&](const uint8_t* codes, uint4 (&w)[kLoads]) {
+#pragma unroll
+      for (int j = 0; j < kRowsEach; ++j)
+#pragma unroll
+        for (int x = 0; x < kPanels; ++x)
+          w[j * kPanels + x] = at[j] < 0 ? make_uint4(0, 0, 0, 0) : ldg_v4(codes + at[j] + x * 64 + chunk * 16);
+    };
+    const auto store = [&](uint8_t* dst, const uint4 (&w)[kLoads]) {
+#pragma unroll
+      for (int j = 0; j < kRowsEach; ++j)
+#pragma unroll
+        for (int x = 0; x < kPanels; ++x) {
+          const uint4 c = w[j * kPanels + x];
+          uint4 a, b;
+          codes_to_half<CODE>(c.x, a.x, a.y);
+          codes_to_half<CODE>(c.y, a.z, a.w);
+          codes_to_half<CODE>(c.z, b.x, b.y);
+          codes_to_half<CODE>(c.w, b.z, b.w);
+          const int rr = tid / 4 + 32 * j;
+          *reinterpret_cast<uint4*>(dst + x * kPanel + swizzled(rr, 2 * chunk)) = a;
+          *reinterpret_cast<uint4*>(dst + x * kPanel + swizzled(rr, 2 * chunk + 1)) = b;
+        }
+    };
+    const auto done = [&](uint64_t* bar) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    float largest = -INFINITY;
+    uint4 kw[kLoads], vw[kLoads];
+    if (count > 0) {
+      locate(0);
+      load(p.k_codes, kw);
+    }
+    for (int i = 0; i < count; ++i) {
+      const int stage = i & 1;
+      const uint32_t parity = ((i >> 1) & 1) ^ 1;
+      load(p.v_codes, vw);
+      if (i >= 2 && !wait(&ctl.k_free[stage], parity, kSiteTransform)) break;
+      if (warp == kSoftmaxWarps) {
+        // the tile's blocks; its place in the ring was last read two products
+        // before the one whose end has just been waited for
+        const int token = token0 + i * kTileTokens + 16 * lane;
+        const int64_t block = lane < kGroups ? block_of(token) : -1;
+        const float ks = block < 0 ? 0.0f : __ldg(p.k_scale + block) * code_gain<CODE>();
+        float lv = block < 0 ? -INFINITY
+                             : __log2f(value_scale(__ldg(p.v_scale + block))) + (CODE == kCodeE4M3 ? 8.0f : 0.0f);
+        float top = lv < 256.0f ? lv : -INFINITY;
+#pragma unroll
+        for (int d = 1; d < kGroups; d *= 2) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
+        top = __shfl_sync(kFullMask, top, 0);
+        largest = fmaxf(largest, top);
+        if (block >= 0 && lv < largest - 64.0f) lv = largest - 64.0f;
+        const float ref = fmaxf(top, largest - 64.0f);
+        const unsigned present = __ballot_sync(kFullMask, block >= 0);
+        if (lane < kGroups) ctl.info[i & 3][lane] = {ks, lv, block < 0 ? 0.0f : exp2_approx(ref - lv)};
+        if (lane == 0) {
+          ctl.top_lv[i & 3] = ref == -INFINITY ? 0.0f : ref;
+          ctl.present[i & 3] = present;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.info_full[i & 3]);
+      }
+      store(smem + Shared::kOffK + stage * Shared::kTile, kw);
+      done(&ctl.k_full[stage]);
+      if (i + 1 < count) {
+        locate(i + 1);
+        load(p.k_codes, kw);
+      }
+      if (i >= 2 && !wait(&ctl.v_free[stage], parity, kSiteTransform)) break;
+      store(smem + Shared::kOffV + stage * Shared::kTile, vw);
+      done(&ctl.v_full[stage]);
+    }
+  } else {
+    // ------------------------------------------------------- softmax
+    const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
+    const uint32_t s_col = tmem + lanes + tile * 128, o_col = tmem + lanes + 256 + tile * 128;
+    float m = -INFINITY, n = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int i = 0; i < count; ++i) {
+      ok = wait(&ctl.info_full[i & 3], (i >> 2) & 1, kSiteEpilogue) &&
+           wait(&ctl.s_full[tile], i & 1, kSiteEpilogue);
+      if (!ok) break;
+      tc_fence_after();
+      const GroupInfo* info = ctl.info[i & 3];
+      const uint32_t present = ctl.present[i & 3];
+      const int base = token0 + i * kTileTokens;
+      // every row of this warp sees every token of the tile
+      const bool whole = __all_sync(kFullMask, lo <= base && base + kTileTokens <= hi) && present == 0xffu;
+
+      float top_t = -INFINITY, top_u = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t s[32];
+        tmem_ld32(s_col + 32 * c, s);
+        tmem_ld_wait(s);
+        uint32_t seen = 0xffffffffu;
+        if (!whole) {
+          seen = bit_range(lo - base - 32 * c, hi - base - 32 * c);
+          if (!(present >> (2 * c) & 1)) seen &= 0xffff0000u;
+          if (!(present >> (2 * c + 1) & 1)) seen &= 0x0000ffffu;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float top = -INFINITY;
+          if (whole) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = fmaxf(top, __uint_as_float(s[16 * h + j]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              top = fmaxf(top, seen >> (16 * h + j) & 1 ? __uint_as_float(s[16 * h + j]) : -INFINITY);
+          }
+          const GroupInfo g = info[2 * c + h];
+          const float u = top == -INFINITY ? -INFINITY : top * (qs * g.ks);
+          top_u = fmaxf(top_u, u);
+          top_t = fmaxf(top_t, u + g.lv);
+        }
+      }
+      // rescale the sums of the rows whose maximum grew by enough
+      const bool grown = top_t > m + kRescaleLog2 || (m == -INFINITY && top_t > m);
+      if (__any_sync(kFullMask, grown)) {
+        const float next = fmaxf(m, top_t), alpha = weight_of(m, next);
+        m = next;
+        if (i > 0) {
+#pragma unroll
+          for (int c = 0; c < DIM / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o_col + 32 * c, o);
+            tmem_ld_wait(o);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+            tmem_st32(o_col + 32 * c, o);
+          }
+          tmem_st_wait();
+        }
+      }
+      const float ref = m == -INFINITY ? 0.0f : m;
+      const float next_n = fmaxf(n, top_u), ref_n = next_n == -INFINITY ? 0.0f : next_n;
+      float sum = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t s[32], w[16];
+        tmem_ld32(s_col + 32 * c, s);
+        tmem_ld_wait(s);
+        uint32_t seen = 0xffffffffu;
+        if (!whole) {
+          seen = bit_range(lo - base - 32 * c, hi - base - 32 * c);
+          if (!(present >> (2 * c) & 1)) seen &= 0xffff0000u;
+          if (!(present >> (2 * c + 1) & 1)) seen &= 0x0000ffffu;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const GroupInfo g = info[2 * c + h];
+          const float a = qs * g.ks, b = g.lv - ref;
+          float part = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            float x = exp2_approx(fmaf(__uint_as_float(s[16 * h + j]), a, b));
+            float y = exp2_approx(fmaf(__uint_as_float(s[16 * h + j + 1]), a, b));
+            if (!whole) {
+              x = seen >> (16 * h + j) & 1 ? x : 0.0f;
+              y = seen >> (16 * h + j + 1) & 1 ? y : 0.0f;
+            }
+            part += x + y;
+            w[8 * h + j / 2] = pack_half2(x, y);
+          }
+          sum = fmaf(part, g.iv, sum);
+        }
+        tmem_st16(s_col + 16 * c, w);
+      }
+      l = fmaf(l, weight_of(n, next_n), sum == 0.0f ? 0.0f : sum * exp2_approx(ref - ctl.top_lv[i & 3] - ref_n));
+      n = next_n;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.p_full[tile]);
+    }
+    if (ok && count > 0) ok = wait(&ctl.o_done[tile], (count - 1) & 1, kSiteEpilogue);
+    if (ok) {
+      tc_fence_after();
+      const float inv = l == 0.0f ? 0.0f : exp2_approx(m - n) / l;
+      const int64_t out_row = output_row(p, blk.s, head, r);
+      float* sums = nullptr;
+      if (parts > 1) {
+        const int64_t part = (slot * p.kv_heads + head) * tp.splits + split;
+        const int rr = tile * kTileRows + row;
+        sums = tp.partial + (part * kCtaRows + rr) * DIM;
+        float* stats = tp.partial + tp.slots * p.kv_heads * tp.splits * kCtaRows * DIM + part * 3 * kCtaRows + rr;
+        stats[0] = m;
+        stats[kCtaRows] = n;
+        stats[2 * kCtaRows] = l;
+      } else if (valid && p.lse != nullptr) {
+        p.lse[out_row] = l == 0.0f ? -INFINITY : (n + __log2f(l)) * kLn2;
+      }
+#pragma unroll
+      for (int c = 0; c < DIM / 32; ++c) {
+        uint32_t o[32];
+        if (count > 0) {
+          tmem_ld32(o_col + 32 * c, o);
+          tmem_ld_wait(o);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0;
+        }
+        if (sums != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<uint4*>(sums + 32 * c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+        } else if (valid) {
+          uint16_t* dst = static_cast<uint16_t*>(p.out) + out_row * DIM + 32 * c;
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            float f[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(o[j + x]) * inv;
+            *reinterpret_cast<uint4*>(dst + j) = p.q_bf16 ? Vec<__nv_bfloat16>::pack(f) : Vec<__half>::pack(f);
+          }
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+// Joins the parts of row blocks that were split: a thread 4 channels of a row.
+constexpr int kJoinThreads = 256;
+
+template <int DIM>
+__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(TilesParams tp) {
+  constexpr int kRowsEach = kJoinThreads / (DIM / 4);
+  const AttendParams& p = tp.a;
+  const int64_t item = blockIdx.x / (kCtaRows / kRowsEach);
+  const int head = static_cast<int>(item % p.kv_heads);
+  const int64_t slot = item / p.kv_heads;
+  Block blk;
+  if (!load_block(p, slot, blk)) return;
+  const int parts = part_count(tp, blk.tiles);
+  const int rr = blockIdx.x % (kCtaRows / kRowsEach) * kRowsEach + threadIdx.x / (DIM / 4);
+  const int64_t r = blk.row0 + rr;
+  if (parts == 1 || r >= blk.rows) return;
+  const int d = threadIdx.x % (DIM / 4) * 4;
+  const int64_t part0 = item * tp.splits;
+  const float* stats = tp.partial + tp.slots * p.kv_heads * tp.splits * kCtaRows * DIM + part0 * 3 * kCtaRows + rr;
+  float m = -INFINITY, n = -INFINITY, l = 0.0f;
+  for (int i = 0; i < parts; ++i) {
+    m = fmaxf(m, stats[i * 3 * kCtaRows]);
+    n = fmaxf(n, stats[i * 3 * kCtaRows + kCtaRows]);
+  }
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int i = 0; i < parts; ++i) {
+    const float w = weight_of(stats[i * 3 * kCtaRows], m);
+    l = fmaf(stats[i * 3 * kCtaRows + 2 * kCtaRows], weight_of(stats[i * 3 * kCtaRows + kCtaRows], n), l);
+    const float4 x = *reinterpret_cast<const float4*>(tp.partial + ((part0 + i) * kCtaRows + rr) * DIM + d);
+    v.x = fmaf(x.x, w, v.x), v.y = fmaf(x.y, w, v.y), v.z = fmaf(x.z, w, v.z), v.w = fmaf(x.w, w, v.w);
+  }
+  const float inv = l == 0.0f ? 0.0f : exp2_approx(m - n) / l;
+  const int64_t out_row = output_row(p, blk.s, head, r);
+  uint2 w;
+  if (p.q_bf16) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x * inv, v.y * inv);
+    const __nv_bfloat162 c = __floats2bfloat162_rn(v.z * inv, v.w * inv);
+    w = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
+  } else {
+    w = make_uint2(pack_half2(v.x * inv, v.y * inv), pack_half2(v.z * inv, v.w * inv));
+  }
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + out_row * DIM + d) = w;
+  if (p.lse != nullptr && d == 0) p.lse[out_row] = l == 0.0f ? -INFINITY : (n + __log2f(l)) * kLn2;
+}
+
+int64_t block_slots(int64_t tokens, int64_t batch, int64_t group) { return tokens * group / kCtaRows + batch; }
+
+// One part while the row blocks alone fill the device; else as many as fill
+// it, with four tiles a part at least at the longest that the table holds.
+int tile_splits(int64_t tokens, int64_t batch, int64_t group, int64_t kv_heads, int64_t width, int page) {
+  const int64_t items = block_slots(tokens, batch, group) * kv_heads;
+  const int64_t most = ceil_div64(ceil_div64(width * page, kTileTokens), 4);
+  const int64_t want = device_sm_count() / items;
+  const int64_t splits = want < most ? want : most;
+  return splits > 1 ? static_cast<int>(splits) : 1;
+}
+
+template <int DIM, int CODE>
+cudaError_t launch_tiles(const TilesParams& tp, cudaStream_t stream) {
+  constexpr int kBytes = kTilesBytes<DIM>;
+  static_assert(kBytes <= 227 * 1024, "a tile's operands do not fit in shared memory");
+  const int64_t items = tp.slots * tp.a.kv_heads;
+  if (items * tp.splits > INT32_MAX) return cudaErrorInvalidValue;
+  static const cudaError_t ready =
+      cudaFuncSetAttribute(kv_tiles_kernel<DIM, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+  if (ready != cudaSuccess) return ready;
+  kv_tiles_kernel<DIM, CODE><<<static_cast<unsigned>(items * tp.splits), kTilesThreads, kBytes, stream>>>(tp);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || tp.splits == 1) return e;
+  constexpr int kBlocks = kCtaRows / (kJoinThreads / (DIM / 4));
+  kv_join_kernel<DIM><<<static_cast<unsigned>(items * kBlocks), kJoinThreads, 0, stream>>>(tp);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t tiles_workspace_bytes(int64_t tokens, int64_t batch, int64_t group, int64_t kv_heads, int dim, int64_t width,
+                             int page) {
+  const int splits = tile_splits(tokens, batch, group, kv_heads, width, page);
+  if (splits == 1) return 0;
+  return static_cast<size_t>(block_slots(tokens, batch, group) * kv_heads * splits) * kCtaRows * (dim + 3) *
+         sizeof(float);
+}
+
+cudaError_t run_tiles(const AttendParams& p, int dim, int code, void* workspace, cudaStream_t stream) {
+  TilesParams tp{};
+  tp.a = p;
+  tp.slots = block_slots(p.tok.tokens, p.tok.batch, p.group);
+  tp.splits = tile_splits(p.tok.tokens, p.tok.batch, p.group, p.kv_heads, p.width, 1 << p.page_shift);
+  tp.partial = static_cast<float*>(workspace);
+  tp.status = status_word_ptr();
+  if (dim == 64)
+    return code == kCodeInt8 ? launch_tiles<64, kCodeInt8>(tp, stream) : launch_tiles<64, kCodeE4M3>(tp, stream);
+  return code == kCodeInt8 ? launch_tiles<128, kCodeInt8>(tp, stream) : launch_tiles<128, kCodeE4M3>(tp, stream);
+}
+
+}  // namespace b2
