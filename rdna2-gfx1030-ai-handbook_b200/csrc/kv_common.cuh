@@ -218,13 +218,14 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t
   }
 }
 
-// fp32 -> one code, round to nearest even, saturating.
+// fp32 -> one code, round to nearest even, saturating; no code is NaN (a NaN
+// shows by its block's scale).
 template <int CODE>
 __device__ __forceinline__ uint32_t to_code(float x) {
   if constexpr (CODE == kCodeInt8) {
     return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(x, -127.0f), 127.0f))) & 0xffu;
   } else {
-    return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+    return __nv_cvt_float_to_fp8(fminf(fmaxf(x, -448.0f), 448.0f), __NV_SATFINITE, __NV_E4M3);
   }
 }
 

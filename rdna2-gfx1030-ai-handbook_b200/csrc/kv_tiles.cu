@@ -14,11 +14,21 @@
 //   warp 12         issues the products: S_t = Q_t K^T (both operands in
 //                   shared memory) and O_t += P_t V (P_t in tensor memory, V
 //                   as stored: its channels are the contiguous dimension)
+//   warp 13         the scales of the next tiles' blocks
+//   warps 14, 15    nothing: registers are shared out by groups of four warps
 //
 // The two row tiles alternate on the tensor cores: while one is in its
-// softmax the other multiplies.  O_t stays in tensor memory and is rescaled
-// only when a row's maximum has grown by more than 2^8 since the last time:
-// weights up to 2^8 are fp16 numbers as good as those up to 1.
+// softmax the other multiplies.  A softmax is one pass and looks for no
+// maximum: weights are taken relative to that of the row's first tile, which
+// fp16 allows while they stay below kMostWeight.  Where a tile's weights sum
+// to more, and where a row has no reference yet, the tile's maxima are found,
+// O_t is rescaled in tensor memory and the tile is gone through once more.
+//
+// int8 keys become operands without their sign: u = c + 128 in the low byte
+// of a half is the (subnormal) number u 2^-24, and the score is
+// q . u - 128 sum(q), a term of the row that the exponent's product takes in.
+// The sums do not cancel much: |u| is at most 255, like the codes' spread.
+// Values are converted to c itself, whose sums may cancel to any degree.
 #include "../../include/b2_attention.h"
 #include "b2_internal.h"
 #include "kv_attention.cuh"
@@ -31,16 +41,19 @@ constexpr int kCtaRows = 2 * kTileRows;
 constexpr int kTileTokens = 128;
 constexpr int kGroups = kTileTokens / 16;   // a group of 16 tokens is in one block, whatever the page
 constexpr int kSoftmaxWarps = 8, kConvertWarps = 4;
-constexpr int kConvertThreads = kConvertWarps * kWarp;
-constexpr int kTilesThreads = (kSoftmaxWarps + kConvertWarps + 1) * kWarp;
-constexpr float kRescaleLog2 = 8.0f;
+constexpr int kMmaWarp = 12, kInfoWarp = 13;
+constexpr int kTilesThreads = 16 * kWarp;
+// Registers a thread: 128 at launch, 2 * 168 + 112 + 64 = 4 * 128 afterwards.
+constexpr int kSoftmaxRegs = 168, kConvertRegs = 112, kOtherRegs = 64;
+constexpr float kMostWeight = 8192.0f;
+constexpr uint32_t kMinusInf = 0xff800000u;
 
 // One row tile of queries, or one tile of K or V: panels of 64 channels, 128
 // rows of 128 bytes each, 128-byte swizzle.
 constexpr int kPanel = 128 * 128;
 
-struct GroupInfo {
-  float ks, lv, iv;  // key scale, log2 of the value scale, 2^(top_lv - lv)
+struct __align__(16) GroupInfo {
+  float ks, lv, iv, unused;  // key scale, log2 of the value scale, 2^(top_lv - lv)
 };
 
 template <int DIM>
@@ -61,6 +74,12 @@ struct TilesControl {
   uint32_t tmem;
   int abort, drained;
 };
+
+// Gain of the products over the codes' own.
+template <int CODE>
+__device__ __forceinline__ float key_gain() {
+  return CODE == kCodeInt8 ? 16777216.0f : 1.0f;
+}
 
 template <int DIM>
 constexpr int kTilesBytes = TilesShared<DIM>::kOffCtl + static_cast<int>(sizeof(TilesControl)) + 1024;
@@ -130,6 +149,35 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Two fp32 numbers in a register pair.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void unpair(uint64_t d, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // Bits [lo, hi) of a word.
 __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
   lo = max(lo, 0);
@@ -138,7 +186,24 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
   return (hi == 32 ? 0xffffffffu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
 }
 
-template <int DIM, int CODE>
+// Four codes -> four halves: keys (int8 as u 2^-24, see above) and values.
+template <int CODE, bool KEYS>
+__device__ __forceinline__ void to_operand(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (CODE == kCodeE4M3) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  } else if constexpr (KEYS) {
+    const uint32_t u = w ^ 0x80808080u;
+    lo = __byte_perm(u, 0u, 0x4140);
+    hi = __byte_perm(u, 0u, 0x4342);
+  } else {
+    codes_to_half<CODE>(w, lo, hi);
+  }
+}
+
+// SEG: tokens that share a block whatever the page, 16 or 64.
+template <int DIM, int CODE, int SEG>
 __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams tp) {
   using Shared = TilesShared<DIM>;
   constexpr int kPanels = DIM / 64;
@@ -162,7 +227,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
   const int count = min(per, blk.tiles - first);
   const int token0 = (blk.tile0 + first) * kTileTokens;
 
-  if (warp == 12) {
+  if (warp == kMmaWarp) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&ctl.k_full[i], kConvertWarps);
@@ -184,7 +249,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
   }
 
   // ---- queries: a softmax thread brings its own row
-  float qs = 0.0f;
+  float qs = 0.0f, bias = 0.0f;  // the scores' factor, and what int8 keys add to their products
   int lo = 0, hi = 0;
   const int tile = warp / 4, row = threadIdx.x % kTileRows;
   const int64_t r = blk.row0 + tile * kTileRows + row;
@@ -220,7 +285,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
         Vec<__half>::unpack(v[c], f);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] *= factor;
+      for (int i = 0; i < 8; ++i) {
+        f[i] *= factor;
+        if (CODE == kCodeInt8) bias = fmaf(__half2float(__float2half_rn(f[i])), -128.0f, bias);
+      }
       *reinterpret_cast<uint4*>(dst + c / 8 * kPanel + swizzled(row, c % 8)) = Vec<__half>::pack(f);
     }
     fence_proxy_async_smem();
@@ -235,7 +303,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
     return __all_sync(kFullMask, mbar_wait(bar, parity, abort_flag, site, tp.status));
   };
 
-  if (warp == 12) {
+  // The block of the cache that holds `token` for this head, or -1.
+  const auto block_of = [&](int token) -> int64_t {
+    if (token >= blk.s.hi) return -1;
+    const int64_t page = __ldg(p.table + static_cast<int64_t>(blk.b) * p.width + (token >> p.page_shift));
+    return page >= 0 && page < p.pages ? page * p.kv_heads + head : -1;
+  };
+  if (warp >= kMmaWarp) fewer_registers<kOtherRegs>();
+  if (warp == kMmaWarp) {
     // ------------------------------------------------------- products
     constexpr uint32_t kIdescS = make_idesc<kKindF16>(kTileRows, kTileTokens);
     constexpr uint32_t kIdescO = make_idesc<kKindF16>(kTileRows, DIM) | (1u << 16);  // V: N contiguous
@@ -301,45 +376,87 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
     commit(&ctl.last);
     mbar_wait(&ctl.last, 0, &ctl.drained, kSiteMma, tp.status);
     __syncwarp();
-  } else if (warp >= kSoftmaxWarps) {
+  } else if (warp == kInfoWarp) {
+    // ------------------------------------------------------- blocks' scales
+    // a lane a group of 16 tokens; the ring's place for tile i was last read
+    // by the softmax of tile i - 4, whose end the products of tile i - 2 need
+    int64_t block = lane < kGroups ? block_of(token0 + 16 * lane) : -1;
+    float ks = 0.0f, vs = 0.0f, largest = -INFINITY;
+    const auto load = [&] {
+      ks = block < 0 ? 0.0f : __ldg(p.k_scale + block);
+      vs = block < 0 ? 0.0f : __ldg(p.v_scale + block);
+    };
+    load();
+    for (int i = 0; i < count; ++i) {
+      const bool here = block >= 0;
+      float lv = here ? __log2f(value_scale(vs)) : -INFINITY;
+      float top = lv < 256.0f ? lv : -INFINITY;
+#pragma unroll
+      for (int d = 1; d < kGroups; d *= 2) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
+      top = __shfl_sync(kFullMask, top, 0);
+      largest = fmaxf(largest, top);
+      if (here && lv < largest - 64.0f) lv = largest - 64.0f;
+      const float ref = fmaxf(top, largest - 64.0f);
+      const unsigned present = __ballot_sync(kFullMask, here);
+      const GroupInfo info = {ks, lv, here ? exp2_approx(ref - lv) : 0.0f, 0.0f};
+      block = lane < kGroups && i + 1 < count ? block_of(token0 + (i + 1) * kTileTokens + 16 * lane) : -1;
+      load();
+      if (i >= 2 && !wait(&ctl.k_free[i & 1], ((i >> 1) & 1) ^ 1, kSiteTransform)) break;
+      if (lane < kGroups) ctl.info[i & 3][lane] = info;
+      if (lane == 0) {
+        ctl.top_lv[i & 3] = ref == -INFINITY ? 0.0f : ref;
+        ctl.present[i & 3] = present;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.info_full[i & 3]);
+    }
+  } else if (warp / 4 == kSoftmaxWarps / 4) {
     // ------------------------------------------------------- codes to fp16
+    // Each operand's codes are loaded as soon as the one before it has left
+    // the registers, and the pages of a tile a tile ahead of that.
+    fewer_registers<kConvertRegs>();
     constexpr int kLoads = DIM / 16;       // 16-byte pieces of a tile a thread takes
     constexpr int kRowsEach = 4;
     const int tid = threadIdx.x - kSoftmaxWarps * kWarp;
     const int chunk = tid % 4;             // quarter-warps take two rows: no bank conflicts below
-    int64_t at[kRowsEach];                 // where this thread's rows begin in the codes, or -1
     const int page_mask = (1 << p.page_shift) - 1;
-    const auto block_of = [&](int token) -> int64_t {
-      if (token >= blk.s.hi) return -1;
-      const int64_t page = __ldg(p.table + static_cast<int64_t>(blk.b) * p.width + (token >> p.page_shift));
-      return page >= 0 && page < p.pages ? page * p.kv_heads + head : -1;
-    };
+    int64_t block[kRowsEach];              // of this thread's rows in the next tile
     const auto locate = [&](int i) {
 #pragma unroll
-      for (int j = 0; j < kRowsEach; ++j) {
-        const int token = token0 + i * kTileTokens + tid / 4 + 32 * j;
-        const int64_t block = block_of(token & ~15);
-        at[j] = block < 0 ? -1 : ((block << p.page_shift) + (token & page_mask)) * DIM;
-      }
+      for (int j = 0; j < kRowsEach; ++j)
+        block[j] = i < count ? block_of(token0 + i * kTileTokens + tid / 4 + 32 * j) : -1;
     };
-    const auto load = [&](const uint8_t* codes, uint4 (&w)[kLoads]) {
+    // where the rows begin in the codes, or -1
+    const auto place = [&](int64_t (&at)[kRowsEach]) {
+#pragma unroll
+      for (int j = 0; j < kRowsEach; ++j)
+        at[j] = block[j] < 0 ? -1 : ((block[j] << p.page_shift) + ((tid / 4 + 32 * j) & page_mask)) * DIM + chunk * 16;
+    };
+    const auto load = [&](const uint8_t* codes, const int64_t (&at)[kRowsEach], uint4 (&w)[kLoads]) {
 #pragma unroll
       for (int j = 0; j < kRowsEach; ++j)
 #pragma unroll
         for (int x = 0; x < kPanels; ++x)
-          w[j * kPanels + x] = at[j] < 0 ? make_uint4(0, 0, 0, 0) : ldg_v4(codes + at[j] + x * 64 + chunk * 16);
+          w[j * kPanels + x] = at[j] < 0 ? make_uint4(0, 0, 0, 0) : ldg_v4(codes + at[j] + x * 64);
     };
-    const auto store = [&](uint8_t* dst, const uint4 (&w)[kLoads]) {
+    const auto store = [&](bool keys, uint8_t* dst, const uint4 (&w)[kLoads]) {
 #pragma unroll
       for (int j = 0; j < kRowsEach; ++j)
 #pragma unroll
         for (int x = 0; x < kPanels; ++x) {
           const uint4 c = w[j * kPanels + x];
           uint4 a, b;
-          codes_to_half<CODE>(c.x, a.x, a.y);
-          codes_to_half<CODE>(c.y, a.z, a.w);
-          codes_to_half<CODE>(c.z, b.x, b.y);
-          codes_to_half<CODE>(c.w, b.z, b.w);
+          if (keys) {
+            to_operand<CODE, true>(c.x, a.x, a.y);
+            to_operand<CODE, true>(c.y, a.z, a.w);
+            to_operand<CODE, true>(c.z, b.x, b.y);
+            to_operand<CODE, true>(c.w, b.z, b.w);
+          } else {
+            to_operand<CODE, false>(c.x, a.x, a.y);
+            to_operand<CODE, false>(c.y, a.z, a.w);
+            to_operand<CODE, false>(c.z, b.x, b.y);
+            to_operand<CODE, false>(c.w, b.z, b.w);
+          }
           const int rr = tid / 4 + 32 * j;
           *reinterpret_cast<uint4*>(dst + x * kPanel + swizzled(rr, 2 * chunk)) = a;
           *reinterpret_cast<uint4*>(dst + x * kPanel + swizzled(rr, 2 * chunk + 1)) = b;
@@ -350,56 +467,34 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    float largest = -INFINITY;
     uint4 kw[kLoads], vw[kLoads];
-    if (count > 0) {
-      locate(0);
-      load(p.k_codes, kw);
-    }
+    int64_t at[kRowsEach];
+    locate(0);
+    place(at);
+    load(p.k_codes, at, kw);
+    load(p.v_codes, at, vw);
+    locate(1);
     for (int i = 0; i < count; ++i) {
       const int stage = i & 1;
       const uint32_t parity = ((i >> 1) & 1) ^ 1;
-      load(p.v_codes, vw);
+      place(at);  // of tile i + 1
+      locate(i + 2);
       if (i >= 2 && !wait(&ctl.k_free[stage], parity, kSiteTransform)) break;
-      if (warp == kSoftmaxWarps) {
-        // the tile's blocks; its place in the ring was last read two products
-        // before the one whose end has just been waited for
-        const int token = token0 + i * kTileTokens + 16 * lane;
-        const int64_t block = lane < kGroups ? block_of(token) : -1;
-        const float ks = block < 0 ? 0.0f : __ldg(p.k_scale + block) * code_gain<CODE>();
-        float lv = block < 0 ? -INFINITY
-                             : __log2f(value_scale(__ldg(p.v_scale + block))) + (CODE == kCodeE4M3 ? 8.0f : 0.0f);
-        float top = lv < 256.0f ? lv : -INFINITY;
-#pragma unroll
-        for (int d = 1; d < kGroups; d *= 2) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
-        top = __shfl_sync(kFullMask, top, 0);
-        largest = fmaxf(largest, top);
-        if (block >= 0 && lv < largest - 64.0f) lv = largest - 64.0f;
-        const float ref = fmaxf(top, largest - 64.0f);
-        const unsigned present = __ballot_sync(kFullMask, block >= 0);
-        if (lane < kGroups) ctl.info[i & 3][lane] = {ks, lv, block < 0 ? 0.0f : exp2_approx(ref - lv)};
-        if (lane == 0) {
-          ctl.top_lv[i & 3] = ref == -INFINITY ? 0.0f : ref;
-          ctl.present[i & 3] = present;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl.info_full[i & 3]);
-      }
-      store(smem + Shared::kOffK + stage * Shared::kTile, kw);
+      store(true, smem + Shared::kOffK + stage * Shared::kTile, kw);
       done(&ctl.k_full[stage]);
-      if (i + 1 < count) {
-        locate(i + 1);
-        load(p.k_codes, kw);
-      }
+      load(p.k_codes, at, kw);
       if (i >= 2 && !wait(&ctl.v_free[stage], parity, kSiteTransform)) break;
-      store(smem + Shared::kOffV + stage * Shared::kTile, vw);
+      store(false, smem + Shared::kOffV + stage * Shared::kTile, vw);
       done(&ctl.v_full[stage]);
+      load(p.v_codes, at, vw);
     }
-  } else {
+  } else if (warp < kSoftmaxWarps) {
     // ------------------------------------------------------- softmax
+    more_registers<kSoftmaxRegs>();
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
     const uint32_t s_col = tmem + lanes + tile * 128, o_col = tmem + lanes + 256 + tile * 128;
-    float m = -INFINITY, n = -INFINITY, l = 0.0f;
+    // references of t and u; a row that is not one of the sequence needs none
+    float m = valid ? -INFINITY : 0.0f, n = m, l = 0.0f;
     bool ok = true;
     for (int i = 0; i < count; ++i) {
       ok = wait(&ctl.info_full[i & 3], (i >> 2) & 1, kSiteEpilogue) &&
@@ -412,89 +507,104 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
       // every row of this warp sees every token of the tile
       const bool whole = __all_sync(kFullMask, lo <= base && base + kTileTokens <= hi) && present == 0xffu;
 
-      float top_t = -INFINITY, top_u = -INFINITY;
+      // 32 scores at a time, the next ones on their way; -inf where masked
+      const auto fetch = [&](int c, uint32_t (&x)[32]) {
+        tmem_ld_wait(x);
+        if (whole) return;
+        const uint32_t seen = bit_range(lo - base - 32 * c, hi - base - 32 * c) &
+                              ((present >> (2 * c) & 1 ? 0xffffu : 0u) | (present >> (2 * c) & 2 ? 0xffff0000u : 0u));
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t s[32];
-        tmem_ld32(s_col + 32 * c, s);
-        tmem_ld_wait(s);
-        uint32_t seen = 0xffffffffu;
-        if (!whole) {
-          seen = bit_range(lo - base - 32 * c, hi - base - 32 * c);
-          if (!(present >> (2 * c) & 1)) seen &= 0xffff0000u;
-          if (!(present >> (2 * c + 1) & 1)) seen &= 0x0000ffffu;
-        }
+        for (int j = 0; j < 32; ++j) x[j] = seen >> j & 1 ? x[j] : kMinusInf;
+      };
+      // Factor and offset that make u of a product, for one block.  A factor
+      // of zero would make NaN of a masked score.
+      const auto factor = [&](const GroupInfo& g, float& a, float& d) {
+        const float product = qs * g.ks;
+        d = bias * product;
+        a = product * key_gain<CODE>();
+        a = a == 0.0f ? 1.17549435e-38f : a;
+      };
+      uint32_t sc[2][32], w[64];
+      float sum, ref, ref_n;
+      bool raise = __any_sync(kFullMask, m == -INFINITY);
+      for (;;) {
+        if (raise) {
+          float top_t = -INFINITY, top_u = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld32(s_col + 32 * c, sc[0]);
+            fetch(c, sc[0]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float top = -INFINITY;
-          if (whole) {
+            for (int h = 0; h < 2; ++h) {
+              float top = -INFINITY, a, d;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) top = fmaxf(top, __uint_as_float(s[16 * h + j]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              top = fmaxf(top, seen >> (16 * h + j) & 1 ? __uint_as_float(s[16 * h + j]) : -INFINITY);
-          }
-          const GroupInfo g = info[2 * c + h];
-          const float u = top == -INFINITY ? -INFINITY : top * (qs * g.ks);
-          top_u = fmaxf(top_u, u);
-          top_t = fmaxf(top_t, u + g.lv);
-        }
-      }
-      // rescale the sums of the rows whose maximum grew by enough
-      const bool grown = top_t > m + kRescaleLog2 || (m == -INFINITY && top_t > m);
-      if (__any_sync(kFullMask, grown)) {
-        const float next = fmaxf(m, top_t), alpha = weight_of(m, next);
-        m = next;
-        if (i > 0) {
-#pragma unroll
-          for (int c = 0; c < DIM / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(o_col + 32 * c, o);
-            tmem_ld_wait(o);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-            tmem_st32(o_col + 32 * c, o);
-          }
-          tmem_st_wait();
-        }
-      }
-      const float ref = m == -INFINITY ? 0.0f : m;
-      const float next_n = fmaxf(n, top_u), ref_n = next_n == -INFINITY ? 0.0f : next_n;
-      float sum = 0.0f;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t s[32], w[16];
-        tmem_ld32(s_col + 32 * c, s);
-        tmem_ld_wait(s);
-        uint32_t seen = 0xffffffffu;
-        if (!whole) {
-          seen = bit_range(lo - base - 32 * c, hi - base - 32 * c);
-          if (!(present >> (2 * c) & 1)) seen &= 0xffff0000u;
-          if (!(present >> (2 * c + 1) & 1)) seen &= 0x0000ffffu;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const GroupInfo g = info[2 * c + h];
-          const float a = qs * g.ks, b = g.lv - ref;
-          float part = 0.0f;
-#pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            float x = exp2_approx(fmaf(__uint_as_float(s[16 * h + j]), a, b));
-            float y = exp2_approx(fmaf(__uint_as_float(s[16 * h + j + 1]), a, b));
-            if (!whole) {
-              x = seen >> (16 * h + j) & 1 ? x : 0.0f;
-              y = seen >> (16 * h + j + 1) & 1 ? y : 0.0f;
+              for (int j = 0; j < 16; ++j) top = fmaxf(top, __uint_as_float(sc[0][16 * h + j]));
+              const GroupInfo g = info[2 * c + h];
+              factor(g, a, d);
+              const float u = fmaf(top, a, d);
+              top_u = fmaxf(top_u, u);
+              top_t = fmaxf(top_t, u + g.lv);
             }
-            part += x + y;
-            w[8 * h + j / 2] = pack_half2(x, y);
           }
-          sum = fmaf(part, g.iv, sum);
+          const float next = fmaxf(m, top_t), next_n = fmaxf(n, top_u), alpha = weight_of(m, next);
+          l *= weight_of(n, next_n);
+          m = next;
+          n = next_n;
+          if (i > 0) {
+#pragma unroll 1
+            for (int c = 0; c < DIM / 32; ++c) {
+              tmem_ld32(o_col + 32 * c, sc[0]);
+              tmem_ld_wait(sc[0]);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) sc[0][j] = __float_as_uint(__uint_as_float(sc[0][j]) * alpha);
+              tmem_st32(o_col + 32 * c, sc[0]);
+            }
+          }
         }
-        tmem_st16(s_col + 16 * c, w);
+        ref = m == -INFINITY ? 0.0f : m;
+        ref_n = n == -INFINITY ? 0.0f : n;
+        float weights = 0.0f;
+        sum = 0.0f;
+        tmem_ld32(s_col, sc[0]);
+#pragma unroll
+        for (int x = 0; x < kTileTokens / SEG; ++x) {
+          const GroupInfo g = info[x * (SEG / 16)];
+          float a, d;
+          factor(g, a, d);
+          d += g.lv - ref;
+          const uint64_t aa = pair_of(a, a), dd = pair_of(d, d);
+          uint64_t part = 0;
+#pragma unroll
+          for (int y = 0; y < SEG; y += 2) {
+            const int at = x * SEG + y, c = at / 32;
+            if (at % 32 == 0) {
+              fetch(c, sc[c & 1]);
+              if (c < 3) tmem_ld32(s_col + 32 * (c + 1), sc[(c + 1) & 1]);
+            }
+            const uint32_t* two = &sc[c & 1][at % 32];
+            float v0, v1;
+            unpair(fma_pair(pair_of(__uint_as_float(two[0]), __uint_as_float(two[1])), aa, dd), v0, v1);
+            v0 = exp2_approx(v0);
+            v1 = exp2_approx(v1);
+            part = add_pair(part, pair_of(v0, v1));
+            w[at / 2] = pack_half2(v0, v1);
+          }
+          float even, odd;
+          unpair(part, even, odd);
+          weights += even + odd;
+          sum = fmaf(even + odd, g.iv, sum);
+        }
+        if (raise || !__any_sync(kFullMask, weights > kMostWeight)) break;
+        raise = true;
       }
-      l = fmaf(l, weight_of(n, next_n), sum == 0.0f ? 0.0f : sum * exp2_approx(ref - ctl.top_lv[i & 3] - ref_n));
-      n = next_n;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t part[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) part[j] = w[16 * c + j];
+        tmem_st16(s_col + 16 * c, part);
+      }
+      l = fmaf(sum, exp2_approx(ref - ctl.top_lv[i & 3] - ref_n), l);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -546,7 +656,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
 // Joins the parts of row blocks that were split: a thread 4 channels of a row.
@@ -606,21 +716,26 @@ int tile_splits(int64_t tokens, int64_t batch, int64_t group, int64_t kv_heads, 
   return splits > 1 ? static_cast<int>(splits) : 1;
 }
 
-template <int DIM, int CODE>
+template <int DIM, int CODE, int SEG>
 cudaError_t launch_tiles(const TilesParams& tp, cudaStream_t stream) {
   constexpr int kBytes = kTilesBytes<DIM>;
   static_assert(kBytes <= 227 * 1024, "a tile's operands do not fit in shared memory");
   const int64_t items = tp.slots * tp.a.kv_heads;
   if (items * tp.splits > INT32_MAX) return cudaErrorInvalidValue;
   static const cudaError_t ready =
-      cudaFuncSetAttribute(kv_tiles_kernel<DIM, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+      cudaFuncSetAttribute(kv_tiles_kernel<DIM, CODE, SEG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
   if (ready != cudaSuccess) return ready;
-  kv_tiles_kernel<DIM, CODE><<<static_cast<unsigned>(items * tp.splits), kTilesThreads, kBytes, stream>>>(tp);
+  kv_tiles_kernel<DIM, CODE, SEG><<<static_cast<unsigned>(items * tp.splits), kTilesThreads, kBytes, stream>>>(tp);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || tp.splits == 1) return e;
   constexpr int kBlocks = kCtaRows / (kJoinThreads / (DIM / 4));
   kv_join_kernel<DIM><<<static_cast<unsigned>(items * kBlocks), kJoinThreads, 0, stream>>>(tp);
   return cudaGetLastError();
+}
+
+template <int DIM, int CODE>
+cudaError_t launch_tiles_page(const TilesParams& tp, cudaStream_t stream) {
+  return tp.a.page_shift >= 6 ? launch_tiles<DIM, CODE, 64>(tp, stream) : launch_tiles<DIM, CODE, 16>(tp, stream);
 }
 
 }  // namespace
@@ -640,9 +755,10 @@ cudaError_t run_tiles(const AttendParams& p, int dim, int code, void* workspace,
   tp.splits = tile_splits(p.tok.tokens, p.tok.batch, p.group, p.kv_heads, p.width, 1 << p.page_shift);
   tp.partial = static_cast<float*>(workspace);
   tp.status = status_word_ptr();
+  const bool int8 = code == kCodeInt8;
   if (dim == 64)
-    return code == kCodeInt8 ? launch_tiles<64, kCodeInt8>(tp, stream) : launch_tiles<64, kCodeE4M3>(tp, stream);
-  return code == kCodeInt8 ? launch_tiles<128, kCodeInt8>(tp, stream) : launch_tiles<128, kCodeE4M3>(tp, stream);
+    return int8 ? launch_tiles_page<64, kCodeInt8>(tp, stream) : launch_tiles_page<64, kCodeE4M3>(tp, stream);
+  return int8 ? launch_tiles_page<128, kCodeInt8>(tp, stream) : launch_tiles_page<128, kCodeE4M3>(tp, stream);
 }
 
 }  // namespace b2
