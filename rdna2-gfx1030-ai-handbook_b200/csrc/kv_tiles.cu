@@ -5,20 +5,22 @@
 // head's query heads -- as two row tiles of 128, and walks the cached tokens
 // they see in tiles of 128.  Roles:
 //
-//   warps 0-3, 4-7  softmax of row tile 0 and 1, a thread a row: scores come
-//                   from tensor memory, weights go back there as fp16 over
-//                   the scores' own columns
-//   warps 8-11      codes -> fp16 operands in shared memory (128-byte swizzle),
+//   warps 0-7, 8-15 softmax of row tile 0 and 1, two threads a row with 64
+//                   tokens each: scores come from tensor memory, weights go
+//                   back there as fp16 over the scores' own columns
+//   warps 16-23     codes -> fp16 operands in shared memory (128-byte swizzle),
 //                   two tiles of K and V each; every operand serves both row
 //                   tiles, so a code is converted once for 256 rows
-//   warp 12         issues the products: S_t = Q_t K^T (both operands in
-//                   shared memory) and O_t += P_t V (P_t in tensor memory, V
-//                   as stored: its channels are the contiguous dimension)
-//   warp 13         the scales of the next tiles' blocks
-//   warps 14, 15    nothing: registers are shared out by groups of four warps
+//   warps 24, 25    issue the products of row tile 0 and 1: S_t = Q_t K^T (both
+//                   operands in shared memory) and O_t += P_t V (P_t in tensor
+//                   memory, V as stored: its channels are contiguous)
+//   warp 26         the scales of the next tiles' blocks
+//   warp 27         nothing: registers are shared out by groups of four warps
 //
 // The two row tiles alternate on the tensor cores: while one is in its
-// softmax the other multiplies.  A softmax is one pass and looks for no
+// softmax the other multiplies, and they take turns so that it stays that way
+// (left alone they fall into step, exponentials and products in turn for
+// both).  A softmax is one pass and looks for no
 // maximum: weights are taken relative to that of the row's first tile, which
 // fp16 allows while they stay below kMostWeight.  Where a tile's weights sum
 // to more, and where a row has no reference yet, the tile's maxima are found,
@@ -40,11 +42,12 @@ constexpr int kTileRows = 128;              // rows of one product (UMMA M)
 constexpr int kCtaRows = 2 * kTileRows;
 constexpr int kTileTokens = 128;
 constexpr int kGroups = kTileTokens / 16;   // a group of 16 tokens is in one block, whatever the page
-constexpr int kSoftmaxWarps = 8, kConvertWarps = 4;
-constexpr int kMmaWarp = 12, kInfoWarp = 13;
-constexpr int kTilesThreads = 16 * kWarp;
-// Registers a thread: 128 at launch, 2 * 168 + 112 + 64 = 4 * 128 afterwards.
-constexpr int kSoftmaxRegs = 168, kConvertRegs = 112, kOtherRegs = 64;
+constexpr int kSoftmaxWarps = 16, kConvertWarps = 8;
+constexpr int kMmaWarp = kSoftmaxWarps + kConvertWarps, kInfoWarp = kMmaWarp + 2;
+constexpr int kTilesThreads = 28 * kWarp;
+// Registers a thread: 72 at launch, 4 * 80 + 2 * 64 + 56 = 7 * 72 afterwards.
+constexpr int kSoftmaxRegs = 80, kConvertRegs = 64, kOtherRegs = 56;
+constexpr int kHalfTokens = kTileTokens / 2;  // of a softmax thread
 constexpr float kMostWeight = 8192.0f;
 constexpr uint32_t kMinusInf = 0xff800000u;
 
@@ -65,12 +68,31 @@ struct TilesShared {
   static constexpr int kOffCtl = kOffV + 2 * kTile;
 };
 
+// A row block and the token tiles that any of its rows sees.
+struct Block {
+  Sequence s;
+  int b;
+  int64_t row0, rows;   // its first row, and the rows of the sequence
+  int tile0, tiles;
+};
+
+// What a CTA works on.  It is kept in shared memory: a softmax thread has no
+// registers to spare, and spilled ones would be fetched past the codes that
+// stream through the first-level cache.
+struct Work {
+  Block blk;
+  int64_t slot;
+  int head, split, parts;
+};
+
 struct TilesControl {
   uint64_t k_full[2], k_free[2], v_full[2], v_free[2];
-  uint64_t s_full[2], p_full[2], o_done[2], info_full[4], last;
+  uint64_t s_full[2], p_full[2], o_done[2], info_full[4], turn[2], last[2];
   GroupInfo info[4][kGroups];
   float top_lv[4];
   uint32_t present[4];  // bit g: group g lies on a page of the cache
+  Work work;
+  float row[2][2][kCtaRows];  // what the two threads of a row tell each other
   uint32_t tmem;
   int abort, drained;
 };
@@ -96,14 +118,6 @@ struct TilesParams {
 __device__ __forceinline__ int64_t first_block(const AttendParams& p, int b) {
   return static_cast<int64_t>(p.tok.begin(b)) * p.group / kCtaRows + b;
 }
-
-// A row block and the token tiles that any of its rows sees.
-struct Block {
-  Sequence s;
-  int b;
-  int64_t row0, rows;   // its first row, and the rows of the sequence
-  int tile0, tiles;
-};
 
 __device__ __forceinline__ bool load_block(const AttendParams& p, int64_t slot, Block& k) {
   k.b = warp_search(p.tok.batch, slot, [&](int i) { return first_block(p, i); });
@@ -140,12 +154,20 @@ __device__ __forceinline__ uint64_t channels_desc(uint32_t saddr) {
          (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
 
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+// 32 columns of this thread's row, complete: loading and waiting in one
+// statement leaves the registers where the load put them.
+__device__ __forceinline__ void tmem_read32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
       : "memory");
 }
 
@@ -215,31 +237,39 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
 
   // the heaviest blocks of a causal prompt, its last rows, come first
-  const int64_t unit = blockIdx.x;
-  const int split = static_cast<int>(unit % tp.splits);
-  const int head = static_cast<int>(unit / tp.splits % p.kv_heads);
-  const int64_t slot = tp.slots - 1 - unit / tp.splits / p.kv_heads;
-  Block blk;
-  if (!load_block(p, slot, blk)) return;
-  const int per = part_tiles(tp, blk.tiles), parts = part_count(tp, blk.tiles);
-  if (split >= parts) return;
-  const int first = split * per;
-  const int count = min(per, blk.tiles - first);
-  const int token0 = (blk.tile0 + first) * kTileTokens;
+  int count, token0;
+  {
+    const int64_t unit = blockIdx.x;
+    Work mine;
+    mine.split = static_cast<int>(unit % tp.splits);
+    mine.head = static_cast<int>(unit / tp.splits % p.kv_heads);
+    mine.slot = tp.slots - 1 - unit / tp.splits / p.kv_heads;
+    if (!load_block(p, mine.slot, mine.blk)) return;
+    mine.parts = part_count(tp, mine.blk.tiles);
+    if (mine.split >= mine.parts) return;
+    const int per = part_tiles(tp, mine.blk.tiles), first = mine.split * per;
+    count = min(per, mine.blk.tiles - first);
+    token0 = (mine.blk.tile0 + first) * kTileTokens;
+    if (threadIdx.x == 0) ctl.work = mine;
+  }
+  __syncthreads();
+  const Work& work = ctl.work;
+  const Block& blk = work.blk;
 
   if (warp == kMmaWarp) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&ctl.k_full[i], kConvertWarps);
         mbar_init(&ctl.v_full[i], kConvertWarps);
-        mbar_init(&ctl.k_free[i], 1);
-        mbar_init(&ctl.v_free[i], 1);
+        mbar_init(&ctl.k_free[i], 2);
+        mbar_init(&ctl.v_free[i], 2);
         mbar_init(&ctl.s_full[i], 1);
-        mbar_init(&ctl.p_full[i], 4);
+        mbar_init(&ctl.p_full[i], kSoftmaxWarps / 2);
         mbar_init(&ctl.o_done[i], 1);
+        mbar_init(&ctl.turn[i], kSoftmaxWarps / 2);
+        mbar_init(&ctl.last[i], 1);
       }
       for (int i = 0; i < 4; ++i) mbar_init(&ctl.info_full[i], 1);
-      mbar_init(&ctl.last, 1);
       ctl.abort = ctl.drained = 0;
       fence_mbar_init();
     }
@@ -248,49 +278,55 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
     tmem_relinquish();
   }
 
-  // ---- queries: a softmax thread brings its own row
-  float qs = 0.0f, bias = 0.0f;  // the scores' factor, and what int8 keys add to their products
-  int lo = 0, hi = 0;
-  const int tile = warp / 4, row = threadIdx.x % kTileRows;
-  const int64_t r = blk.row0 + tile * kTileRows + row;
-  const bool valid = warp < kSoftmaxWarps && r < blk.rows;
+  // ---- queries: a softmax thread brings half of its row's channels
+  const int tile = warp / 8, half = warp / 4 % 2, row = threadIdx.x % kTileRows;
+  const int cta_row = tile * kTileRows + row;
+  constexpr int kChunks = DIM / 16;  // 16-byte pieces of half a row
+  uint4 qv[kChunks];
   if (warp < kSoftmaxWarps) {
-    uint4 v[DIM / 8];
+    const int64_t r = blk.row0 + cta_row;
+    const bool valid = r < blk.rows;
     uint32_t top = 0;
     const uint16_t* src = static_cast<const uint16_t*>(p.q) + (blk.s.first + r / p.group) * p.q_token +
-                          (head * p.group + r % p.group) * p.q_head;
+                          (work.head * p.group + r % p.group) * p.q_head + half * (DIM / 2);
 #pragma unroll
-    for (int c = 0; c < DIM / 8; ++c) {
-      v[c] = valid ? ldg_v4(src + 8 * c) : make_uint4(0, 0, 0, 0);
+    for (int c = 0; c < kChunks; ++c) {
+      qv[c] = valid ? ldg_v4(src + 8 * c) : make_uint4(0, 0, 0, 0);
       float f[8];
       if (p.q_bf16) {
-        Vec<__nv_bfloat16>::unpack(v[c], f);
+        Vec<__nv_bfloat16>::unpack(qv[c], f);
       } else {
-        Vec<__half>::unpack(v[c], f);
+        Vec<__half>::unpack(qv[c], f);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
     }
-    float factor, gain;
-    row_power(top, factor, gain);
+    ctl.row[0][half][cta_row] = __uint_as_float(top);
+  }
+  __syncthreads();
+  float qs = 0.0f;
+  if (warp < kSoftmaxWarps) {
+    float factor, gain, sum = 0.0f;
+    row_power(max(__float_as_uint(ctl.row[0][0][cta_row]), __float_as_uint(ctl.row[0][1][cta_row])), factor, gain);
     qs = gain * p.scale_log2;
-    if (valid) row_bounds(p, blk.s, blk.s.start + r / p.group, lo, hi);
     uint8_t* dst = smem + Shared::kOffQ + tile * Shared::kTile;
 #pragma unroll
-    for (int c = 0; c < DIM / 8; ++c) {
+    for (int c = 0; c < kChunks; ++c) {
       float f[8];
       if (p.q_bf16) {
-        Vec<__nv_bfloat16>::unpack(v[c], f);
+        Vec<__nv_bfloat16>::unpack(qv[c], f);
       } else {
-        Vec<__half>::unpack(v[c], f);
+        Vec<__half>::unpack(qv[c], f);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         f[i] *= factor;
-        if (CODE == kCodeInt8) bias = fmaf(__half2float(__float2half_rn(f[i])), -128.0f, bias);
+        sum += __half2float(__float2half_rn(f[i]));
       }
-      *reinterpret_cast<uint4*>(dst + c / 8 * kPanel + swizzled(row, c % 8)) = Vec<__half>::pack(f);
+      const int chunk = half * kChunks + c;
+      *reinterpret_cast<uint4*>(dst + chunk / 8 * kPanel + swizzled(row, chunk % 8)) = Vec<__half>::pack(f);
     }
+    ctl.row[1][half][cta_row] = sum;
     fence_proxy_async_smem();
   }
   tc_fence_before();
@@ -307,14 +343,15 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
   const auto block_of = [&](int token) -> int64_t {
     if (token >= blk.s.hi) return -1;
     const int64_t page = __ldg(p.table + static_cast<int64_t>(blk.b) * p.width + (token >> p.page_shift));
-    return page >= 0 && page < p.pages ? page * p.kv_heads + head : -1;
+    return page >= 0 && page < p.pages ? page * p.kv_heads + work.head : -1;
   };
   if (warp >= kMmaWarp) fewer_registers<kOtherRegs>();
-  if (warp == kMmaWarp) {
+  if (warp == kMmaWarp || warp == kMmaWarp + 1) {
     // ------------------------------------------------------- products
     constexpr uint32_t kIdescS = make_idesc<kKindF16>(kTileRows, kTileTokens);
     constexpr uint32_t kIdescO = make_idesc<kKindF16>(kTileRows, DIM) | (1u << 16);  // V: N contiguous
-    const auto scores = [&](int t, int stage) {
+    const int t = warp - kMmaWarp;
+    const auto scores = [&](int stage) {
       if (elect_one()) {
         const uint32_t q = base_u32 + Shared::kOffQ + t * Shared::kTile;
         const uint32_t k = base_u32 + Shared::kOffK + stage * Shared::kTile;
@@ -324,57 +361,44 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
           umma<kKindF16>(tmem + t * 128, sw128_desc(q + off), sw128_desc(k + off), kIdescS, x > 0);
         }
         umma_commit(&ctl.s_full[t]);
+        umma_commit(&ctl.k_free[stage]);
       }
       __syncwarp();
     };
-    const auto output = [&](int t, int stage, bool add) {
+    const auto output = [&](int stage, bool add) {
       if (elect_one()) {
         const uint32_t v = base_u32 + Shared::kOffV + stage * Shared::kTile;
 #pragma unroll
         for (int x = 0; x < kTileTokens / 16; ++x)
           umma_ts_f16(tmem + 256 + t * 128, tmem + t * 128 + 8 * x, channels_desc(v + x * 2048), kIdescO, add || x > 0);
         umma_commit(&ctl.o_done[t]);
+        umma_commit(&ctl.v_free[stage]);
       }
       __syncwarp();
     };
-    const auto commit = [&](uint64_t* bar) {
-      if (elect_one()) umma_commit(bar);
-      __syncwarp();
-    };
-    bool ok = true;
-    if (count > 0) {
-      ok = wait(&ctl.k_full[0], 0, kSiteMma);
-      if (ok) {
-        tc_fence_after();
-        scores(0, 0);
-        scores(1, 0);
-        commit(&ctl.k_free[0]);
-      }
+    bool ok = count == 0 || wait(&ctl.k_full[0], 0, kSiteMma);
+    if (ok && count > 0) {
+      tc_fence_after();
+      scores(0);
     }
     for (int i = 0; ok && i < count; ++i) {
-      const int stage = i & 1, next = stage ^ 1;
-      const uint32_t parity = (i >> 1) & 1, next_parity = ((i + 1) >> 1) & 1;
-      ok = wait(&ctl.v_full[stage], parity, kSiteMma);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (!ok || !(ok = wait(&ctl.p_full[t], i & 1, kSiteMma))) break;
+      ok = wait(&ctl.v_full[i & 1], (i >> 1) & 1, kSiteMma) && wait(&ctl.p_full[t], i & 1, kSiteMma);
+      if (!ok) break;
+      tc_fence_after();
+      output(i & 1, i > 0);
+      if (i + 1 < count) {
+        // the weights lie where the next scores go: they have been read first
+        ok = wait(&ctl.k_full[(i + 1) & 1], ((i + 1) >> 1) & 1, kSiteMma) && wait(&ctl.o_done[t], i & 1, kSiteMma);
+        if (!ok) break;
         tc_fence_after();
-        output(t, stage, i > 0);
-        if (t == 1) commit(&ctl.v_free[stage]);
-        if (i + 1 < count) {
-          // the weights lie where the next scores go: they have been read first
-          ok = (t == 1 || wait(&ctl.k_full[next], next_parity, kSiteMma)) && wait(&ctl.o_done[t], i & 1, kSiteMma);
-          if (!ok) break;
-          tc_fence_after();
-          scores(t, next);
-          if (t == 1) commit(&ctl.k_free[next]);
-        }
+        scores((i + 1) & 1);
       }
     }
     // nothing is in flight when tensor memory is given back, after a wait
     // that gave up either
-    commit(&ctl.last);
-    mbar_wait(&ctl.last, 0, &ctl.drained, kSiteMma, tp.status);
+    if (elect_one()) umma_commit(&ctl.last[t]);
+    __syncwarp();
+    mbar_wait(&ctl.last[t], 0, &ctl.drained, kSiteMma, tp.status);
     __syncwarp();
   } else if (warp == kInfoWarp) {
     // ------------------------------------------------------- blocks' scales
@@ -410,27 +434,27 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.info_full[i & 3]);
     }
-  } else if (warp / 4 == kSoftmaxWarps / 4) {
+  } else if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
     // ------------------------------------------------------- codes to fp16
     // Each operand's codes are loaded as soon as the one before it has left
     // the registers, and the pages of a tile a tile ahead of that.
     fewer_registers<kConvertRegs>();
-    constexpr int kLoads = DIM / 16;       // 16-byte pieces of a tile a thread takes
-    constexpr int kRowsEach = 4;
+    constexpr int kRowsEach = 2;
+    constexpr int kLoads = kRowsEach * kPanels;  // 16-byte pieces of a tile a thread takes
     const int tid = threadIdx.x - kSoftmaxWarps * kWarp;
-    const int chunk = tid % 4;             // quarter-warps take two rows: no bank conflicts below
+    const int chunk = tid % 4;                   // quarter-warps take two rows: no bank conflicts below
     const int page_mask = (1 << p.page_shift) - 1;
-    int64_t block[kRowsEach];              // of this thread's rows in the next tile
+    int64_t block[kRowsEach];                    // of this thread's rows in the next tile
     const auto locate = [&](int i) {
 #pragma unroll
       for (int j = 0; j < kRowsEach; ++j)
-        block[j] = i < count ? block_of(token0 + i * kTileTokens + tid / 4 + 32 * j) : -1;
+        block[j] = i < count ? block_of(token0 + i * kTileTokens + tid / 4 + 64 * j) : -1;
     };
     // where the rows begin in the codes, or -1
     const auto place = [&](int64_t (&at)[kRowsEach]) {
 #pragma unroll
       for (int j = 0; j < kRowsEach; ++j)
-        at[j] = block[j] < 0 ? -1 : ((block[j] << p.page_shift) + ((tid / 4 + 32 * j) & page_mask)) * DIM + chunk * 16;
+        at[j] = block[j] < 0 ? -1 : ((block[j] << p.page_shift) + ((tid / 4 + 64 * j) & page_mask)) * DIM + chunk * 16;
     };
     const auto load = [&](const uint8_t* codes, const int64_t (&at)[kRowsEach], uint4 (&w)[kLoads]) {
 #pragma unroll
@@ -457,7 +481,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
             to_operand<CODE, false>(c.z, b.x, b.y);
             to_operand<CODE, false>(c.w, b.z, b.w);
           }
-          const int rr = tid / 4 + 32 * j;
+          const int rr = tid / 4 + 64 * j;
           *reinterpret_cast<uint4*>(dst + x * kPanel + swizzled(rr, 2 * chunk)) = a;
           *reinterpret_cast<uint4*>(dst + x * kPanel + swizzled(rr, 2 * chunk + 1)) = b;
         }
@@ -492,24 +516,37 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
     // ------------------------------------------------------- softmax
     more_registers<kSoftmaxRegs>();
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
-    const uint32_t s_col = tmem + lanes + tile * 128, o_col = tmem + lanes + 256 + tile * 128;
+    const uint32_t s_col = tmem + lanes + tile * 128 + half * kHalfTokens;         // this thread's scores,
+    const uint32_t p_col = tmem + lanes + tile * 128 + half * (kHalfTokens / 2);   // weights
+    const uint32_t o_col = tmem + lanes + 256 + tile * 128 + half * (DIM / 2);     // and channels
+    const int pair = 1 + tile * 4 + warp % 4;  // named barrier of the two warps that share rows
+    const int other = half ^ 1;
+    // what int8 keys without their sign add to a row's products
+    const float bias = CODE == kCodeInt8 ? -128.0f * (ctl.row[1][0][cta_row] + ctl.row[1][1][cta_row]) : 0.0f;
+    int lo = 0, hi = 0;
     // references of t and u; a row that is not one of the sequence needs none
-    float m = valid ? -INFINITY : 0.0f, n = m, l = 0.0f;
+    float m = 0.0f, n = 0.0f, l = 0.0f;
+    if (blk.row0 + cta_row < blk.rows) {
+      row_bounds(p, blk.s, blk.s.start + (blk.row0 + cta_row) / p.group, lo, hi);
+      m = n = -INFINITY;
+    }
     bool ok = true;
     for (int i = 0; i < count; ++i) {
       ok = wait(&ctl.info_full[i & 3], (i >> 2) & 1, kSiteEpilogue) &&
-           wait(&ctl.s_full[tile], i & 1, kSiteEpilogue);
+           wait(&ctl.s_full[tile], i & 1, kSiteEpilogue) &&
+           (i + tile == 0 || wait(&ctl.turn[tile], (i + tile - 1) & 1, kSiteEpilogue));
+      ok = bar_and(pair, 2 * kWarp, ok);
       if (!ok) break;
       tc_fence_after();
-      const GroupInfo* info = ctl.info[i & 3];
-      const uint32_t present = ctl.present[i & 3];
-      const int base = token0 + i * kTileTokens;
-      // every row of this warp sees every token of the tile
-      const bool whole = __all_sync(kFullMask, lo <= base && base + kTileTokens <= hi) && present == 0xffu;
+      const GroupInfo* info = ctl.info[i & 3] + half * (kHalfTokens / 16);
+      const uint32_t present = ctl.present[i & 3] >> (half * (kHalfTokens / 16));
+      const int base = token0 + i * kTileTokens + half * kHalfTokens;
+      // every row of this warp sees every one of its tokens
+      const bool whole = __all_sync(kFullMask, lo <= base && base + kHalfTokens <= hi) && (present & 0xfu) == 0xfu;
 
-      // 32 scores at a time, the next ones on their way; -inf where masked
+      // 32 scores; -inf where masked
       const auto fetch = [&](int c, uint32_t (&x)[32]) {
-        tmem_ld_wait(x);
+        tmem_read32(s_col + 32 * c, x);
         if (whole) return;
         const uint32_t seen = bit_range(lo - base - 32 * c, hi - base - 32 * c) &
                               ((present >> (2 * c) & 1 ? 0xffffu : 0u) | (present >> (2 * c) & 2 ? 0xffff0000u : 0u));
@@ -524,21 +561,21 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
         a = product * key_gain<CODE>();
         a = a == 0.0f ? 1.17549435e-38f : a;
       };
-      uint32_t sc[2][32], w[64];
+      uint32_t w[kHalfTokens / 2];
       float sum, ref, ref_n;
-      bool raise = __any_sync(kFullMask, m == -INFINITY);
+      bool raise = i == 0, last = true;  // last: the turn has not been passed on
       for (;;) {
         if (raise) {
           float top_t = -INFINITY, top_u = -INFINITY;
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            tmem_ld32(s_col + 32 * c, sc[0]);
-            fetch(c, sc[0]);
+          for (int c = 0; c < kHalfTokens / 32; ++c) {
+            uint32_t sc[32];
+            fetch(c, sc);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float top = -INFINITY, a, d;
 #pragma unroll
-              for (int j = 0; j < 16; ++j) top = fmaxf(top, __uint_as_float(sc[0][16 * h + j]));
+              for (int j = 0; j < 16; ++j) top = fmaxf(top, __uint_as_float(sc[16 * h + j]));
               const GroupInfo g = info[2 * c + h];
               factor(g, a, d);
               const float u = fmaf(top, a, d);
@@ -546,18 +583,23 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
               top_t = fmaxf(top_t, u + g.lv);
             }
           }
-          const float next = fmaxf(m, top_t), next_n = fmaxf(n, top_u), alpha = weight_of(m, next);
+          ctl.row[0][half][cta_row] = top_t;
+          ctl.row[1][half][cta_row] = top_u;
+          named_bar_sync(pair, 2 * kWarp);
+          const float next = fmaxf(m, fmaxf(top_t, ctl.row[0][other][cta_row]));
+          const float next_n = fmaxf(n, fmaxf(top_u, ctl.row[1][other][cta_row]));
+          const float alpha = weight_of(m, next);
           l *= weight_of(n, next_n);
           m = next;
           n = next_n;
           if (i > 0) {
 #pragma unroll 1
-            for (int c = 0; c < DIM / 32; ++c) {
-              tmem_ld32(o_col + 32 * c, sc[0]);
-              tmem_ld_wait(sc[0]);
+            for (int c = 0; c < DIM / 64; ++c) {
+              uint32_t o[32];
+              tmem_read32(o_col + 32 * c, o);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) sc[0][j] = __float_as_uint(__uint_as_float(sc[0][j]) * alpha);
-              tmem_st32(o_col + 32 * c, sc[0]);
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+              tmem_st32(o_col + 32 * c, o);
             }
           }
         }
@@ -565,9 +607,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
         ref_n = n == -INFINITY ? 0.0f : n;
         float weights = 0.0f;
         sum = 0.0f;
-        tmem_ld32(s_col, sc[0]);
+        uint32_t sc[32];
 #pragma unroll
-        for (int x = 0; x < kTileTokens / SEG; ++x) {
+        for (int x = 0; x < kHalfTokens / SEG; ++x) {
           const GroupInfo g = info[x * (SEG / 16)];
           float a, d;
           factor(g, a, d);
@@ -576,12 +618,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
           uint64_t part = 0;
 #pragma unroll
           for (int y = 0; y < SEG; y += 2) {
-            const int at = x * SEG + y, c = at / 32;
-            if (at % 32 == 0) {
-              fetch(c, sc[c & 1]);
-              if (c < 3) tmem_ld32(s_col + 32 * (c + 1), sc[(c + 1) & 1]);
-            }
-            const uint32_t* two = &sc[c & 1][at % 32];
+            const int at = x * SEG + y;
+            if (at % 32 == 0) fetch(at / 32, sc);
+            // the other row tile's turn, with its first steps under these
+            if (at == 32 && last && lane == 0) mbar_arrive(&ctl.turn[tile ^ 1]);
+            const uint32_t* two = &sc[at % 32];
             float v0, v1;
             unpair(fma_pair(pair_of(__uint_as_float(two[0]), __uint_as_float(two[1])), aa, dd), v0, v1);
             v0 = exp2_approx(v0);
@@ -594,16 +635,16 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
           weights += even + odd;
           sum = fmaf(even + odd, g.iv, sum);
         }
-        if (raise || !__any_sync(kFullMask, weights > kMostWeight)) break;
+        // both threads of a row go on, or both raise its reference; weights
+        // may lie where the other one's scores were
+        tc_fence_before();
+        const bool fits = raise || (weights <= kMostWeight && m > -INFINITY) || weights != weights;
+        if (bar_and(pair, 2 * kWarp, fits)) break;
         raise = true;
+        last = false;
       }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t part[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) part[j] = w[16 * c + j];
-        tmem_st16(s_col + 16 * c, part);
-      }
+      tc_fence_after();
+      tmem_st32(p_col, w);
       l = fmaf(sum, exp2_approx(ref - ctl.top_lv[i & 3] - ref_n), l);
       tmem_st_wait();
       tc_fence_before();
@@ -611,28 +652,34 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
       if (lane == 0) mbar_arrive(&ctl.p_full[tile]);
     }
     if (ok && count > 0) ok = wait(&ctl.o_done[tile], (count - 1) & 1, kSiteEpilogue);
+    ctl.row[0][half][cta_row] = l;
+    ok = bar_and(pair, 2 * kWarp, ok);
     if (ok) {
       tc_fence_after();
+      l += ctl.row[0][other][cta_row];
       const float inv = l == 0.0f ? 0.0f : exp2_approx(m - n) / l;
-      const int64_t out_row = output_row(p, blk.s, head, r);
+      const int64_t r = blk.row0 + cta_row;
+      const bool valid = r < blk.rows;
+      const int64_t out_row = output_row(p, blk.s, work.head, r);
       float* sums = nullptr;
-      if (parts > 1) {
-        const int64_t part = (slot * p.kv_heads + head) * tp.splits + split;
-        const int rr = tile * kTileRows + row;
-        sums = tp.partial + (part * kCtaRows + rr) * DIM;
-        float* stats = tp.partial + tp.slots * p.kv_heads * tp.splits * kCtaRows * DIM + part * 3 * kCtaRows + rr;
-        stats[0] = m;
-        stats[kCtaRows] = n;
-        stats[2 * kCtaRows] = l;
-      } else if (valid && p.lse != nullptr) {
+      if (work.parts > 1) {
+        const int64_t part = (work.slot * p.kv_heads + work.head) * tp.splits + work.split;
+        sums = tp.partial + (part * kCtaRows + cta_row) * DIM + half * (DIM / 2);
+        if (half == 0) {
+          float* stats =
+              tp.partial + tp.slots * p.kv_heads * tp.splits * kCtaRows * DIM + part * 3 * kCtaRows + cta_row;
+          stats[0] = m;
+          stats[kCtaRows] = n;
+          stats[2 * kCtaRows] = l;
+        }
+      } else if (half == 0 && valid && p.lse != nullptr) {
         p.lse[out_row] = l == 0.0f ? -INFINITY : (n + __log2f(l)) * kLn2;
       }
-#pragma unroll
-      for (int c = 0; c < DIM / 32; ++c) {
+#pragma unroll 1
+      for (int c = 0; c < DIM / 64; ++c) {
         uint32_t o[32];
         if (count > 0) {
-          tmem_ld32(o_col + 32 * c, o);
-          tmem_ld_wait(o);
+          tmem_read32(o_col + 32 * c, o);
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) o[j] = 0;
@@ -642,7 +689,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
           for (int j = 0; j < 32; j += 4)
             *reinterpret_cast<uint4*>(sums + 32 * c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
         } else if (valid) {
-          uint16_t* dst = static_cast<uint16_t*>(p.out) + out_row * DIM + 32 * c;
+          uint16_t* dst = static_cast<uint16_t*>(p.out) + out_row * DIM + half * (DIM / 2) + 32 * c;
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             float f[8];
