@@ -19,14 +19,24 @@
 //
 // kv_rows_kernel: few query rows.  The rows of one kv head (its query heads
 // times the call's tokens) are the N = 8 or 16 columns of mma.sync m16n8k16
-// and 16 cached tokens its M: the cache is read once, straight from global
-// memory into the operand registers, since a code needs only to be where its
-// product is formed, and products may be formed in any order of channels.
+// and 16 cached tokens its M, so that the cache is read once and nothing is
+// padded to a large tile.  A code needs only to be where its product is
+// formed, and products may be formed in any order of channels and tokens: a
+// lane takes whole 16-byte pieces of rows, and the order of rows is the one
+// that keeps those reads free of bank conflicts.  Every warp has its own ring
+// of 16-token stages, filled by TMA, and its own softmax; the warps of a CTA,
+// and the CTAs that share a (sequence, kv head), are joined at its end.
 #include "../../include/b2_attention.h"
 #include "b2_internal.h"
 #include "kv_attention.cuh"
 
 namespace b2 {
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn tensor_map_encoder();  // qgemm.cu
+
 namespace {
 
 // ----------------------------------------------------------- few query rows
@@ -35,42 +45,100 @@ constexpr int kRowsThreads = kRowsWarps * kWarp;
 constexpr int kRowsTile = 16 * kRowsWarps;  // cached tokens a CTA takes at once
 constexpr int kRowsMaxGrid = 1024;
 
-template <int DIM, int NT>
-struct RowsShared {
-  float sums[kRowsWarps][8 * NT][DIM];
-  float m[kRowsWarps][8 * NT], n[kRowsWarps][8 * NT], l[kRowsWarps][8 * NT];
-  int64_t scan[kRowsWarps];
-  int64_t local;
-  int sequence, last;
+// Stages of a warp's ring, 16 tokens of K and V each: two CTAs of an SM with
+// two, or one with four.
+template <int NT>
+constexpr int kStages = NT == 1 ? 2 : 4;
+
+// A run of token tiles of one item: a sequence, a kv head and 8 * NT rows.
+// Kept in shared memory, the registers being short.
+struct Segment {
+  Sequence s;
+  int b, head, tile0, take, tiles;
+  int64_t row0, rows, local, at;  // `local` and `at`: its first tile within the sequence's and within all
 };
 
-template <int NT>
+template <int DIM, int NT>
+struct __align__(1024) RowsShared {
+  uint8_t ring[kRowsWarps][kStages<NT>][2][16 * DIM];
+  float sums[kRowsWarps][8 * NT][DIM];
+  float m[kRowsWarps][8 * NT], n[kRowsWarps][8 * NT], l[kRowsWarps][8 * NT];
+  uint64_t full[kRowsWarps][kStages<NT>];
+  int block[kRowsWarps][kStages<NT>];  // of a stage's tokens, or -1
+  int64_t scan[kRowsWarps];
+  Segment seg[2];
+  int last, abort;
+};
+
 __device__ __forceinline__ int rows_tiles(const Sequence& s) {
   return max(1, (s.hi + kRowsTile - 1) / kRowsTile - s.lo / kRowsTile);
 }
 
-// Row tiles x heads of a sequence, each with rows_tiles() token tiles.
+__device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint64_t* bar, void* dst, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// Row of a stage that holds the i-th token of each half of 8.  Keys are read
+// by quarter-warps of two rows (i, i + 1), values by t = 0..3 of rows 2t, then
+// of rows 2t + 1; in this order, under the swizzle of the load, neither meets
+// a bank twice.
+template <int DIM>
+__device__ __forceinline__ int stage_row(int i) {
+  return (DIM == 128 ? 0x37156240u : 0x65742130u) >> (4 * i) & 7;
+}
+
+// Byte `at` of row `row` in a stage as the load swizzles it.
+template <int DIM>
+__device__ __forceinline__ uint32_t stage_byte(int row, int at) {
+  return row * DIM + (DIM == 128 ? at ^ ((row & 7) << 4) : at ^ ((row >> 1 & 3) << 4));
+}
+
 template <int NT>
-__device__ __forceinline__ int64_t rows_items(const AttendParams& p, const Sequence& s) {
-  return ceil_div64(static_cast<int64_t>(s.count) * p.group, 8 * NT) * p.kv_heads;
+__device__ __forceinline__ Segment segment_at(const AttendParams& p, const Sequence& s, int b, int64_t local,
+                                              int64_t at, int64_t end) {
+  Segment g;
+  g.s = s;
+  g.b = b;
+  g.local = local;
+  g.at = at;
+  g.rows = static_cast<int64_t>(s.count) * p.group;
+  g.tiles = rows_tiles(s);
+  const int64_t row_tiles = ceil_div64(g.rows, 8 * NT), item = local / g.tiles;
+  g.tile0 = static_cast<int>(local % g.tiles);
+  g.take = static_cast<int>(min(static_cast<int64_t>(g.tiles - g.tile0), end - at));
+  g.head = static_cast<int>(item / row_tiles);
+  g.row0 = item % row_tiles * (8 * NT);
+  return g;
 }
 
 template <int DIM, int CODE, int NT>
-__global__ void __launch_bounds__(kRowsThreads) kv_rows_kernel(AttendParams p) {
-  constexpr int kRows = 8 * NT;
+__global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
+    kv_rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap k_map,
+                   const __grid_constant__ CUtensorMap v_map) {
+  constexpr int kRows = 8 * NT, kRing = kStages<NT>;
   constexpr int kChunks = DIM / 64;  // 16-byte pieces of a key row a lane takes
   constexpr int kVWords = DIM / 32;  // words of a value row a lane takes
-  extern __shared__ __align__(16) uint8_t raw[];
-  RowsShared<DIM, NT>& sh = *reinterpret_cast<RowsShared<DIM, NT>*>(raw);
+  extern __shared__ uint8_t raw[];
+  RowsShared<DIM, NT>& sh =
+      *reinterpret_cast<RowsShared<DIM, NT>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
   const int g = lane / 4, t = lane % 4;
   const int cta = blockIdx.x;
+  if (lane == 0) {
+    for (int i = 0; i < kRing; ++i) mbar_init(&sh.full[warp][i], 1);
+    if (warp == 0) sh.abort = 0;
+    fence_mbar_init();
+  }
 
   // ---- this CTA's share of all (item, token tile) pairs, in order
   const auto cost = [&](int b) -> int64_t {
     if (b >= p.tok.batch) return 0;
     const Sequence s = load_sequence(p, b);
-    return s.count ? rows_items<NT>(p, s) * rows_tiles<NT>(s) : 0;
+    return ceil_div64(static_cast<int64_t>(s.count) * p.group, kRows) * p.kv_heads * rows_tiles(s);
   };
   // inclusive sum over the CTA's threads, and the sum of all
   const auto scan = [&](int64_t v, int64_t& all) -> int64_t {
@@ -105,44 +173,97 @@ __global__ void __launch_bounds__(kRowsThreads) kv_rows_kernel(AttendParams p) {
     int64_t all;
     const int64_t c = cost(base + threadIdx.x), upto = before + scan(c, all);
     if (upto - c <= begin && begin < upto) {
-      sh.sequence = base + threadIdx.x;
-      sh.local = begin - (upto - c);
+      const int b = base + threadIdx.x;
+      sh.seg[0] = segment_at<NT>(p, load_sequence(p, b), b, begin - (upto - c), begin, end);
     }
     before += all;
   }
   __syncthreads();
-  int b = sh.sequence;
-  int64_t local = sh.local;
-  Sequence s = load_sequence(p, b);
 
-  for (int64_t at = begin; at < end;) {
-    const int tiles = rows_tiles<NT>(s);
-    const int64_t row_tiles = ceil_div64(static_cast<int64_t>(s.count) * p.group, kRows);
-    const int64_t item = local / tiles;
-    const int tile0 = static_cast<int>(local % tiles);
-    const int take = static_cast<int>(min(static_cast<int64_t>(tiles - tile0), end - at));
-    const int head = static_cast<int>(item / row_tiles);
-    const int64_t row0 = item % row_tiles * kRows;
-    const int64_t item_begin = at - tile0, item_end = item_begin + tiles;
-    const int64_t rows = static_cast<int64_t>(s.count) * p.group;
+  // ---- this warp's ring, and its groups of the segment at hand
+  uint32_t issued = 0, used = 0;  // stages, ever
+  bool failed = false;            // a wait gave up: no more loads, and no more waits but those for loads in flight
+  int groups = 0, base0 = 0;
+  int next_block = -1;            // of the group that is issued next
+  float next_ks = 0.0f, next_vs = 0.0f;
+  const auto block_at = [&](const Segment& seg, int i) -> int {
+    if (i >= groups) return -1;
+    const int token = base0 + i * kRowsTile;
+    const int page = __ldg(p.table + static_cast<int64_t>(seg.b) * p.width + (token >> p.page_shift));
+    return page >= 0 && page < p.pages ? page * p.kv_heads + seg.head : -1;
+  };
+  const auto issue = [&](int i, int block) {
+    const int stage = issued % kRing;
+    if (lane == 0) {
+      sh.block[warp][stage] = block;
+      uint64_t* bar = &sh.full[warp][stage];
+      if (block >= 0) {
+        const int y = (base0 + i * kRowsTile) & ((1 << p.page_shift) - 1);
+        mbar_arrive_expect_tx(bar, 2 * 16 * DIM);
+        tma_load_3d(&k_map, bar, sh.ring[warp][stage][0], 0, y, block);
+        tma_load_3d(&v_map, bar, sh.ring[warp][stage][1], 0, y, block);
+      } else {
+        mbar_arrive(bar);
+      }
+    }
+    ++issued;
+    __syncwarp();
+  };
+  const auto fetch_scales = [&] {
+    const int block = sh.block[warp][used % kRing];
+    next_ks = block < 0 ? 0.0f : __ldg(p.k_scale + block);
+    next_vs = block < 0 ? 0.0f : __ldg(p.v_scale + block);
+  };
+  const auto start = [&](const Segment& seg) {
+    base0 = (seg.s.lo / kRowsTile + seg.tile0) * kRowsTile + warp * 16;
+    groups = base0 < seg.s.hi && !failed ? min(seg.take, (seg.s.hi - base0 + kRowsTile - 1) / kRowsTile) : 0;
+    int block[kRing];
+#pragma unroll
+    for (int i = 0; i < kRing; ++i) block[i] = block_at(seg, i);
+#pragma unroll
+    for (int i = 0; i < kRing; ++i)
+      if (i < groups) issue(i, block[i]);
+    next_block = block_at(seg, kRing);
+    if (groups > 0) fetch_scales();
+  };
 
+  start(sh.seg[0]);
+  for (int which = 0;; which ^= 1) {
+    const Segment& seg = sh.seg[which];
+    const bool more = seg.at + seg.take < end;
+    if (more && threadIdx.x == kRowsThreads - 1) {  // seen by the others after the barrier below
+      Sequence s = seg.s;
+      int b = seg.b;
+      int64_t local = seg.local + seg.take;
+      if (local == ceil_div64(seg.rows, kRows) * p.kv_heads * seg.tiles) {
+        do {
+          s = load_sequence(p, ++b);
+        } while (s.count == 0);
+        local = 0;
+      }
+      sh.seg[which ^ 1] = segment_at<NT>(p, s, b, local, seg.at + seg.take, end);
+    }
+    __syncwarp();
+    const int64_t row0 = seg.row0, rows = seg.rows;
     // ---- queries: lane (g, t) holds of row g the channels its key chunks hold
     uint32_t qf[NT][kChunks][8];
-    float qs[NT][2], m[NT][2], mu[NT][2], l[NT][2], o[NT][kVWords * 2][4];
-    float largest = -INFINITY;
+    float qa[NT][2], qb[NT][2];  // u = product * qa * ks + qb * ks
+    float m[NT][2], mu[NT][2], l[NT][2], o[NT][kVWords * 2][4];
     int lo[NT][2], hi[NT][2];
+    float largest = -INFINITY;
+    int lo_most = 0, hi_least = INT32_MAX;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int64_t r = row0 + n * 8 + g;
       uint4 raw_q[kChunks][2];
       uint32_t top = 0;
-      float f[kChunks][16];
+      float f[kChunks][16], sum = 0.0f;
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
         raw_q[c][0] = raw_q[c][1] = make_uint4(0, 0, 0, 0);
         if (r < rows) {
-          const uint16_t* row = static_cast<const uint16_t*>(p.q) + (s.first + r / p.group) * p.q_token +
-                                (head * p.group + r % p.group) * p.q_head + (t + 4 * c) * 16;
+          const uint16_t* row = static_cast<const uint16_t*>(p.q) + (seg.s.first + r / p.group) * p.q_token +
+                                (seg.head * p.group + r % p.group) * p.q_head + (t + 4 * c) * 16;
           raw_q[c][0] = ldg_v4(row);
           raw_q[c][1] = ldg_v4(row + 8);
         }
@@ -168,55 +289,86 @@ __global__ void __launch_bounds__(kRowsThreads) kv_rows_kernel(AttendParams p) {
 #pragma unroll
       for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 8; ++i) {
           qf[n][c][i] = pack_half2(f[c][2 * i] * factor, f[c][2 * i + 1] * factor);
+          const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&qf[n][c][i]));
+          sum += h.x + h.y;
+        }
+      sum += __shfl_xor_sync(kFullMask, sum, 1);
+      sum += __shfl_xor_sync(kFullMask, sum, 2);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        qs[n][j] = __shfl_sync(kFullMask, gain, 8 * t + 4 * j) * p.scale_log2;
+        const float qs = __shfl_sync(kFullMask, gain, 8 * t + 4 * j) * p.scale_log2;
+        qa[n][j] = qs * key_gain<CODE>();
+        qb[n][j] = CODE == kCodeInt8 ? -128.0f * __shfl_sync(kFullMask, sum, 8 * t + 4 * j) * qs : 0.0f;
         m[n][j] = mu[n][j] = -INFINITY;
         l[n][j] = 0.0f;
         const int64_t rj = row0 + n * 8 + 2 * t + j;
-        lo[n][j] = hi[n][j] = 0;
-        if (rj < rows) row_bounds(p, s, s.start + rj / p.group, lo[n][j], hi[n][j]);
+        lo[n][j] = 0;
+        hi[n][j] = INT32_MAX;  // a row that is not one of the sequence's: whatever it sums is not stored
+        if (rj < rows) row_bounds(p, seg.s, seg.s.start + rj / p.group, lo[n][j], hi[n][j]);
+        lo_most = max(lo_most, lo[n][j]);
+        hi_least = min(hi_least, hi[n][j]);
       }
 #pragma unroll
       for (int i = 0; i < kVWords * 2; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[n][i][j] = 0.0f;
     }
+    lo_most = __reduce_max_sync(kFullMask, lo_most);
+    hi_least = __reduce_min_sync(kFullMask, hi_least);
 
     // ---- tokens: each warp its own 16 of every tile
-    const int first_tile = s.lo / kRowsTile + tile0;
-    for (int i = 0; i < take; ++i) {
-      const int base = (first_tile + i) * kRowsTile + warp * 16;
-      if (base >= s.hi) break;
-      const int64_t page = __ldg(p.table + static_cast<int64_t>(b) * p.width + (base >> p.page_shift));
-      if (page < 0 || page >= p.pages) continue;
-      const int64_t block = page * p.kv_heads + head;
-      const int64_t byte0 = ((block << p.page_shift) + (base & ((1 << p.page_shift) - 1))) * DIM;
+    const int row_a = stage_row<DIM>(g);                                        // key rows row_a, row_a + 8
+    const int row_b = stage_row<DIM>(2 * t), row_c = stage_row<DIM>(2 * t + 1);  // value rows, and those + 8
+    for (int i = 0; i < groups; ++i) {
+      const int stage = used % kRing, base = base0 + i * kRowsTile;
+      if (!__all_sync(kFullMask, mbar_wait(&sh.full[warp][stage], used / kRing & 1, &sh.abort, kSiteProducer,
+                                           p.status))) {
+        failed = true;
+        break;
+      }
+      ++used;
+      const bool here = sh.block[warp][stage] >= 0;
+      const float ks = next_ks, vs = next_vs;
       uint4 kw[kChunks][2];
       uint32_t vw[4][kVWords];
+      if (here) {
+        const uint32_t k_at = smem_u32(sh.ring[warp][stage][0]), v_at = smem_u32(sh.ring[warp][stage][1]);
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const uint8_t* row = p.k_codes + byte0 + g * DIM + (t + 4 * c) * 16;
-        kw[c][0] = ldg_v4(row);
-        kw[c][1] = ldg_v4(row + 8 * DIM);
-      }
+        for (int c = 0; c < kChunks; ++c) {
+          const uint32_t at = k_at + stage_byte<DIM>(row_a, (t + 4 * c) * 16);
+          kw[c][0] = lds_v4(at);
+          kw[c][1] = lds_v4(at + 8 * DIM);
+        }
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const uint8_t* row = p.v_codes + byte0 + (2 * t + (x & 1) + 8 * (x >> 1)) * DIM + g * (DIM / 8);
-        if constexpr (kVWords == 4) {
-          const uint4 w = ldg_v4(row);
-          vw[x][0] = w.x, vw[x][1] = w.y, vw[x][2] = w.z, vw[x][3] = w.w;
-        } else {
-          const uint2 w = __ldg(reinterpret_cast<const uint2*>(row));
-          vw[x][0] = w.x, vw[x][1] = w.y;
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t at = v_at + stage_byte<DIM>(x & 1 ? row_c : row_b, g * (DIM / 8)) + (x >> 1) * 8 * DIM;
+          if constexpr (kVWords == 4) {
+            const uint4 w = lds_v4(at);
+            vw[x][0] = w.x, vw[x][1] = w.y, vw[x][2] = w.z, vw[x][3] = w.w;
+          } else {
+            lds_v2(at, vw[x][0], vw[x][1]);
+          }
         }
       }
-      const float ks = __ldg(p.k_scale + block) * code_gain<CODE>();
-      const float lv = value_exponent(__ldg(p.v_scale + block), CODE == kCodeE4M3 ? 8.0f : 0.0f, largest);
+      __syncwarp();  // the stage has been read
+      if (i + kRing < groups) {
+        issue(i + kRing, next_block);
+        next_block = block_at(seg, i + kRing + 1);
+      }
+      if (i + 1 < groups) fetch_scales();
+      if (!here) continue;
+      if (base + 16 > seg.s.hi) {  // what lies behind the last token may be no number, and meets weights of zero
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (base + (x & 1 ? row_c : row_b) + 8 * (x >> 1) >= seg.s.hi)
+#pragma unroll
+            for (int w = 0; w < kVWords; ++w) vw[x][w] = 0;
+      }
+      const float lv = value_exponent(vs, 0.0f, largest);
 
-      // scores of tokens g and g + 8 (rows) for query rows 2t and 2t + 1
+      // scores of tokens row_a and row_a + 8 (rows) for query rows 2t and 2t + 1
       float sc[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -229,42 +381,42 @@ __global__ void __launch_bounds__(kRowsThreads) kv_rows_kernel(AttendParams p) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           uint32_t a[4];
-          codes_to_half<CODE>(w0[k], a[0], a[2]);
-          codes_to_half<CODE>(w1[k], a[1], a[3]);
+          to_operand<CODE, true>(w0[k], a[0], a[2]);
+          to_operand<CODE, true>(w1[k], a[1], a[3]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) mma_f16(sc[n], a, qf[n][c][2 * k], qf[n][c][2 * k + 1]);
         }
       }
+      const bool whole = lo_most <= base && base + 16 <= hi_least;
       uint32_t pf[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int col = j & 1, token = base + g + 8 * (j >> 1);
-          const bool seen = token >= lo[n][col] && token < hi[n][col];
-          sc[n][j] = seen ? fmaf(sc[n][j], qs[n][col] * ks, lv) : -INFINITY;
-          top[col] = fmaxf(top[col], sc[n][j]);
-        }
 #pragma unroll
         for (int col = 0; col < 2; ++col) {
+          const float a = qa[n][col] * ks, d = fmaf(qb[n][col], ks, lv);
+          float x = fmaf(sc[n][col], a, d), y = fmaf(sc[n][col + 2], a, d);
+          if (!whole) {
+            const int token = base + row_a;
+            x = token >= lo[n][col] && token < hi[n][col] ? x : -INFINITY;
+            y = token + 8 >= lo[n][col] && token + 8 < hi[n][col] ? y : -INFINITY;
+          }
+          float top = fmaxf(x, y);
 #pragma unroll
-          for (int d = 4; d < kWarp; d *= 2) top[col] = fmaxf(top[col], __shfl_xor_sync(kFullMask, top[col], d));
-          const float next = fmaxf(m[n][col], top[col]);
+          for (int s = 4; s < kWarp; s *= 2) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, s));
+          const float next = fmaxf(m[n][col], top), next_u = fmaxf(mu[n][col], top - lv);
+          const float ref = next == -INFINITY ? 0.0f : next, ref_u = next_u == -INFINITY ? 0.0f : next_u;
           const float alpha = weight_of(m[n][col], next);
-          const float ref = next == -INFINITY ? 0.0f : next;
+          x = exp2_approx(x - ref);
+          y = exp2_approx(y - ref);
+          l[n][col] = fmaf(l[n][col], weight_of(mu[n][col], next_u), (x + y) * exp2_approx(ref - lv - ref_u));
           m[n][col] = next;
-          sc[n][col] = exp2_approx(sc[n][col] - ref);
-          sc[n][col + 2] = exp2_approx(sc[n][col + 2] - ref);
-          const float next_u = fmaxf(mu[n][col], top[col] - lv);
-          const float ref_u = next_u == -INFINITY ? 0.0f : next_u;
-          l[n][col] = fmaf(l[n][col], weight_of(mu[n][col], next_u),
-                           (sc[n][col] + sc[n][col + 2]) * exp2_approx(ref - lv - ref_u));
           mu[n][col] = next_u;
+          sc[n][col] = x;
+          sc[n][col + 2] = y;
 #pragma unroll
-          for (int x = 0; x < kVWords * 2; ++x) {
-            o[n][x][col] *= alpha;
-            o[n][x][col + 2] *= alpha;
+          for (int v = 0; v < kVWords * 2; ++v) {
+            o[n][v][col] *= alpha;
+            o[n][v][col + 2] *= alpha;
           }
         }
         pf[n][0] = transpose_8x8(pack_half2(sc[n][0], sc[n][1]));
@@ -276,19 +428,20 @@ __global__ void __launch_bounds__(kRowsThreads) kv_rows_kernel(AttendParams p) {
         const uint32_t l01 = __byte_perm(vw[0][w], vw[1][w], 0x5140), l23 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
         const uint32_t h01 = __byte_perm(vw[2][w], vw[3][w], 0x5140), h23 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
         uint32_t a[4];
-        codes_to_half<CODE>(l01, a[0], a[1]);
-        codes_to_half<CODE>(h01, a[2], a[3]);
+        to_operand<CODE, false>(l01, a[0], a[1]);
+        to_operand<CODE, false>(h01, a[2], a[3]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * w], a, pf[n][0], pf[n][1]);
-        codes_to_half<CODE>(l23, a[0], a[1]);
-        codes_to_half<CODE>(h23, a[2], a[3]);
+        to_operand<CODE, false>(l23, a[0], a[1]);
+        to_operand<CODE, false>(h23, a[2], a[3]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * w + 1], a, pf[n][0], pf[n][1]);
       }
     }
 
-    // ---- join the warps
+    // ---- join the warps, with the next segment's first loads on their way
     __syncthreads();
+    if (more) start(sh.seg[which ^ 1]);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -320,17 +473,18 @@ __global__ void __launch_bounds__(kRowsThreads) kv_rows_kernel(AttendParams p) {
       }
     __syncthreads();
 
-    const bool whole = take == tiles;
     // CTAs that share the item: the one it begins in and those that follow
+    const int64_t item_begin = seg.at - seg.tile0, item_end = item_begin + seg.tiles;
     const int owner = static_cast<int>(ceil_div64((item_begin + 1) * parts, total) - 1);
-    const int sharers = whole ? 1 : static_cast<int>(ceil_div64(item_end * parts, total) - 1) - owner + 1;
+    const int sharers =
+        seg.take == seg.tiles ? 1 : static_cast<int>(ceil_div64(item_end * parts, total) - 1) - owner + 1;
     constexpr int kSlot = kRows * (DIM + 3);
     float* slot = p.partial + (static_cast<int64_t>(cta) * 2 + (item_begin >= begin ? 1 : 0)) * kSlot;
     const auto store = [&](int64_t r, int d, float4 v, float top, float top_u, float sum) {
       if (r >= rows) return;
       const float inv = sum == 0.0f ? 0.0f : exp2_approx(top - top_u) / sum;
-      const int64_t row = (s.first + r / p.group) * static_cast<int64_t>(p.kv_heads * p.group) + head * p.group +
-                          r % p.group;
+      const int64_t row = (seg.s.first + r / p.group) * static_cast<int64_t>(p.kv_heads * p.group) +
+                          seg.head * p.group + r % p.group;
       uint2 w;
       if (p.q_bf16) {
         const __nv_bfloat162 a = __floats2bfloat162_rn(v.x * inv, v.y * inv);
@@ -404,26 +558,41 @@ __global__ void __launch_bounds__(kRowsThreads) kv_rows_kernel(AttendParams p) {
         }
       }
     }
+    if (!more) break;
     __syncthreads();
-
-    at += take;
-    local += take;
-    if (local == row_tiles * p.kv_heads * tiles && at < end) {
-      do {
-        s = load_sequence(p, ++b);
-      } while (s.count == 0);
-      local = 0;
-    }
   }
+  // after a wait that gave up, loads may still be in flight
+  for (; used != issued; ++used) {
+    volatile int never = 0;
+    mbar_wait(&sh.full[warp][used % kRing], used / kRing & 1, &never, kSiteProducer, p.status);
+  }
+}
+
+// [pages * kv_heads][page][DIM] codes, in boxes of 16 tokens.
+template <int DIM>
+bool encode_codes(CUtensorMap* map, const void* codes, int64_t blocks, int page) {
+  const auto encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[3] = {DIM, static_cast<cuuint64_t>(page), static_cast<cuuint64_t>(blocks)};
+  const cuuint64_t strides[2] = {DIM, static_cast<cuuint64_t>(page) * DIM};
+  const cuuint32_t box[3] = {DIM, 16, 1}, step[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(codes), dims, strides, box, step,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, DIM == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int DIM, int CODE, int NT>
 cudaError_t run_rows(const AttendParams& p, int grid, cudaStream_t stream) {
-  constexpr int kBytes = sizeof(RowsShared<DIM, NT>);
+  constexpr int kBytes = sizeof(RowsShared<DIM, NT>) + 1024;
   static const cudaError_t ready = cudaFuncSetAttribute(
       kv_rows_kernel<DIM, CODE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
   if (ready != cudaSuccess) return ready;
-  kv_rows_kernel<DIM, CODE, NT><<<grid, kRowsThreads, kBytes, stream>>>(p);
+  CUtensorMap k_map{}, v_map{};
+  const int64_t blocks = p.pages * p.kv_heads;
+  if (blocks > 0 && !(encode_codes<DIM>(&k_map, p.k_codes, blocks, 1 << p.page_shift) &&
+                      encode_codes<DIM>(&v_map, p.v_codes, blocks, 1 << p.page_shift)))
+    return cudaErrorInvalidValue;
+  kv_rows_kernel<DIM, CODE, NT><<<grid, kRowsThreads, kBytes, stream>>>(p, k_map, v_map);
   return cudaGetLastError();
 }
 
@@ -502,7 +671,7 @@ int b2_kv_attention(const void* q, int dtype, int64_t tokens, int64_t q_heads, i
   const auto aligned = [](const void* x, uintptr_t n) { return reinterpret_cast<uintptr_t>(x) % n == 0; };
   if ((dtype != b2::kF16 && dtype != b2::kBF16) || code < 0 || code > 1) return invalid;
   if (!b2::shapes_ok(tokens, batch, max_new, q_heads, kv_heads, dim, width, page)) return invalid;
-  if (pages < 0 || pages > INT32_MAX || window < 0 || !(scale > 0.0f) || scale > 3.0e38f) return invalid;
+  if (pages < 0 || pages * kv_heads > INT32_MAX || window < 0 || !(scale > 0.0f) || scale > 3.0e38f) return invalid;
   if (tokens == 0) return 0;
   if (batch < 1 || max_new < 1 || (offsets == nullptr && (tokens % batch || tokens / batch > max_new))) return invalid;
   if (!q || !lengths || (!table && width) || !k_codes || !v_codes || !k_scale || !v_scale || !out) return invalid;
@@ -531,6 +700,7 @@ int b2_kv_attention(const void* q, int dtype, int64_t tokens, int64_t q_heads, i
   p.window = window;
   p.out = out;
   p.lse = lse;
+  p.status = b2::status_word_ptr();
   p.counters = static_cast<int*>(workspace);
   p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + b2::kRowsMaxGrid * sizeof(int));
   if (plan.tiles)

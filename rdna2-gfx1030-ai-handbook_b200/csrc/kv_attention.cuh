@@ -27,6 +27,7 @@ struct AttendParams {
   int64_t window;    // 0: none
   void* out;
   float* lse;
+  int* status;       // the bounded-wait status word
   int* counters;     // [grid], zero between calls
   float* partial;    // [grid][2] slots
 };
@@ -89,6 +90,33 @@ __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// int8 keys become operands without their sign: u = c + 128 in the low byte
+// of a half is the (subnormal) number u 2^-24, and the score is
+// q . u - 128 sum(q), a term of the row that the exponent's product takes in.
+// The sums do not cancel much: u is at most 255, twice the codes' spread.
+// Values are converted to c itself, whose sums may cancel to any degree.
+// Gain of the products over the codes' own.
+template <int CODE>
+__device__ __forceinline__ float key_gain() {
+  return CODE == kCodeInt8 ? 16777216.0f : 1.0f;
+}
+
+// Four codes -> four halves: keys (int8 as u 2^-24, see above) and values.
+template <int CODE, bool KEYS>
+__device__ __forceinline__ void to_operand(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (CODE == kCodeE4M3) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  } else if constexpr (KEYS) {
+    const uint32_t u = w ^ 0x80808080u;
+    lo = __byte_perm(u, 0u, 0x4140);
+    hi = __byte_perm(u, 0u, 0x4342);
+  } else {
+    codes_to_half<CODE>(w, lo, hi);
+  }
 }
 
 // A block that no token was appended to may hold any scale: one at or below

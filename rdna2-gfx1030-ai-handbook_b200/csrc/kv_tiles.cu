@@ -25,12 +25,6 @@
 // fp16 allows while they stay below kMostWeight.  Where a tile's weights sum
 // to more, and where a row has no reference yet, the tile's maxima are found,
 // O_t is rescaled in tensor memory and the tile is gone through once more.
-//
-// int8 keys become operands without their sign: u = c + 128 in the low byte
-// of a half is the (subnormal) number u 2^-24, and the score is
-// q . u - 128 sum(q), a term of the row that the exponent's product takes in.
-// The sums do not cancel much: |u| is at most 255, like the codes' spread.
-// Values are converted to c itself, whose sums may cancel to any degree.
 #include "../../include/b2_attention.h"
 #include "b2_internal.h"
 #include "kv_attention.cuh"
@@ -96,12 +90,6 @@ struct TilesControl {
   uint32_t tmem;
   int abort, drained;
 };
-
-// Gain of the products over the codes' own.
-template <int CODE>
-__device__ __forceinline__ float key_gain() {
-  return CODE == kCodeInt8 ? 16777216.0f : 1.0f;
-}
 
 template <int DIM>
 constexpr int kTilesBytes = TilesShared<DIM>::kOffCtl + static_cast<int>(sizeof(TilesControl)) + 1024;
@@ -206,22 +194,6 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
   hi = min(hi, 32);
   if (lo >= hi) return 0u;
   return (hi == 32 ? 0xffffffffu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
-}
-
-// Four codes -> four halves: keys (int8 as u 2^-24, see above) and values.
-template <int CODE, bool KEYS>
-__device__ __forceinline__ void to_operand(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (CODE == kCodeE4M3) {
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-        : "=r"(lo), "=r"(hi)
-        : "r"(w));
-  } else if constexpr (KEYS) {
-    const uint32_t u = w ^ 0x80808080u;
-    lo = __byte_perm(u, 0u, 0x4140);
-    hi = __byte_perm(u, 0u, 0x4342);
-  } else {
-    codes_to_half<CODE>(w, lo, hi);
-  }
 }
 
 // SEG: tokens that share a block whatever the page, 16 or 64.
