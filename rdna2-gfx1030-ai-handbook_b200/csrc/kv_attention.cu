@@ -82,6 +82,14 @@ __device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint64_t* ba
       : "memory");
 }
 
+// Where channels d .. d + 3 of row r lie while warps are joined: rows 2t (and
+// 2t + 1), which a quarter-warp writes at once, in banks of their own.
+template <int DIM>
+__device__ __forceinline__ int sum_place(int r, int d) {
+  const int t = r >> 1 & 3;
+  return d ^ (DIM == 128 ? t : (t & 1) | (t & 2) << 1) << 2;
+}
+
 // Row of a stage that holds the i-th token of each half of 8.  Keys are read
 // by quarter-warps of two rows (i, i + 1), values by t = 0..3 of rows 2t, then
 // of rows 2t + 1; in this order, under the swizzle of the load, neither meets
@@ -159,10 +167,11 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
     }
     return v + before;
   };
-  int64_t total = 0;
+  int64_t total = 0, first_cost = 0, first_upto = 0;
   for (int base = 0; base < p.tok.batch; base += kRowsThreads) {
     int64_t all;
-    scan(cost(base + threadIdx.x), all);
+    const int64_t c = cost(base + threadIdx.x), upto = scan(c, all);
+    if (base == 0) first_cost = c, first_upto = upto;
     total += all;
   }
   const int64_t parts = min(static_cast<int64_t>(gridDim.x), total);  // CTAs with work: none of them is empty
@@ -170,8 +179,11 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
   const int64_t begin = cta * total / parts, end = (cta + 1) * total / parts;
   int64_t before = 0;
   for (int base = 0; base < p.tok.batch && before <= begin; base += kRowsThreads) {
-    int64_t all;
-    const int64_t c = cost(base + threadIdx.x), upto = before + scan(c, all);
+    int64_t all = 0, c = first_cost, upto = first_upto;
+    if (base > 0 || p.tok.batch > kRowsThreads) {
+      c = cost(base + threadIdx.x);
+      upto = before + scan(c, all);
+    }
     if (upto - c <= begin && begin < upto) {
       const int b = base + threadIdx.x;
       sh.seg[0] = segment_at<NT>(p, load_sequence(p, b), b, begin - (upto - c), begin, end);
@@ -388,9 +400,13 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
         }
       }
       const bool whole = lo_most <= base && base + 16 <= hi_least;
-      uint32_t pf[NT][2];
+      // t of the group's tokens, their weights against the references of
+      // earlier groups, and whether those have to be raised: a row has none
+      // yet, or a weight is above what fp16 should hold
+      bool raise = false;
+      float weight[NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int col = 0; col < 2; ++col) {
           const float a = qa[n][col] * ks, d = fmaf(qb[n][col], ks, lv);
@@ -400,27 +416,47 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
             x = token >= lo[n][col] && token < hi[n][col] ? x : -INFINITY;
             y = token + 8 >= lo[n][col] && token + 8 < hi[n][col] ? y : -INFINITY;
           }
-          float top = fmaxf(x, y);
-#pragma unroll
-          for (int s = 4; s < kWarp; s *= 2) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, s));
-          const float next = fmaxf(m[n][col], top), next_u = fmaxf(mu[n][col], top - lv);
-          const float ref = next == -INFINITY ? 0.0f : next, ref_u = next_u == -INFINITY ? 0.0f : next_u;
-          const float alpha = weight_of(m[n][col], next);
-          x = exp2_approx(x - ref);
-          y = exp2_approx(y - ref);
-          l[n][col] = fmaf(l[n][col], weight_of(mu[n][col], next_u), (x + y) * exp2_approx(ref - lv - ref_u));
-          m[n][col] = next;
-          mu[n][col] = next_u;
           sc[n][col] = x;
           sc[n][col + 2] = y;
-#pragma unroll
-          for (int v = 0; v < kVWords * 2; ++v) {
-            o[n][v][col] *= alpha;
-            o[n][v][col + 2] *= alpha;
-          }
+          const float ref = m[n][col] == -INFINITY ? 0.0f : m[n][col];
+          weight[n][col] = exp2_approx(x - ref);
+          weight[n][col + 2] = exp2_approx(y - ref);
+          raise |= fmaxf(weight[n][col], weight[n][col + 2]) > kMostWeight;
+          raise |= m[n][col] == -INFINITY && fmaxf(x, y) > -INFINITY;
         }
-        pf[n][0] = transpose_8x8(pack_half2(sc[n][0], sc[n][1]));
-        pf[n][1] = transpose_8x8(pack_half2(sc[n][2], sc[n][3]));
+      if (__any_sync(kFullMask, raise)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int col = 0; col < 2; ++col) {
+            float top = fmaxf(sc[n][col], sc[n][col + 2]);
+#pragma unroll
+            for (int s = 4; s < kWarp; s *= 2) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, s));
+            const float next = fmaxf(m[n][col], top), next_u = fmaxf(mu[n][col], top - lv);
+            const float ref = next == -INFINITY ? 0.0f : next, alpha = weight_of(m[n][col], next);
+            l[n][col] *= weight_of(mu[n][col], next_u);
+            m[n][col] = next;
+            mu[n][col] = next_u;
+            weight[n][col] = exp2_approx(sc[n][col] - ref);
+            weight[n][col + 2] = exp2_approx(sc[n][col + 2] - ref);
+#pragma unroll
+            for (int v = 0; v < kVWords * 2; ++v) {
+              o[n][v][col] *= alpha;
+              o[n][v][col + 2] *= alpha;
+            }
+          }
+      }
+      uint32_t pf[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int col = 0; col < 2; ++col) {
+          const float ref = m[n][col] == -INFINITY ? 0.0f : m[n][col];
+          const float ref_u = mu[n][col] == -INFINITY ? 0.0f : mu[n][col];
+          l[n][col] = fmaf(weight[n][col] + weight[n][col + 2], exp2_approx(ref - lv - ref_u), l[n][col]);
+        }
+        pf[n][0] = transpose_8x8(pack_half2(weight[n][0], weight[n][1]));
+        pf[n][1] = transpose_8x8(pack_half2(weight[n][2], weight[n][3]));
       }
       // channels 2x and 2x + 1 of this lane's chunk are output rows g and g + 8
 #pragma unroll
@@ -466,10 +502,10 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
         for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, sh.m[w][r]);
         const float weight = weight_of(m[n][col], top);
 #pragma unroll
-        for (int x = 0; x < kVWords * 2; ++x) {
-          sh.sums[warp][r][g * (DIM / 8) + 2 * x] = o[n][x][col] * weight;
-          sh.sums[warp][r][g * (DIM / 8) + 2 * x + 1] = o[n][x][col + 2] * weight;
-        }
+        for (int x = 0; x < kVWords; ++x)
+          *reinterpret_cast<float4*>(&sh.sums[warp][r][sum_place<DIM>(r, g * (DIM / 8) + 4 * x)]) =
+              make_float4(o[n][2 * x][col] * weight, o[n][2 * x][col + 2] * weight, o[n][2 * x + 1][col] * weight,
+                          o[n][2 * x + 1][col + 2] * weight);
       }
     __syncthreads();
 
@@ -507,7 +543,7 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
       }
 #pragma unroll
       for (int w = 0; w < kRowsWarps; ++w) {
-        const float4 x = *reinterpret_cast<const float4*>(&sh.sums[w][r][d]);
+        const float4 x = *reinterpret_cast<const float4*>(&sh.sums[w][r][sum_place<DIM>(r, d)]);
         v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
         sum = fmaf(sh.l[w][r], weight_of(sh.n[w][r], top_u), sum);
       }

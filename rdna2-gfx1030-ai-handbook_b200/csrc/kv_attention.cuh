@@ -9,6 +9,10 @@ namespace b2 {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// A softmax goes on with the reference it has while its weights (in the tile
+// kernel their sum over a tile) stay below this.
+constexpr float kMostWeight = 8192.0f;
+
 struct AttendParams {
   Tokens tok;
   const void* q;

@@ -42,7 +42,6 @@ constexpr int kTilesThreads = 28 * kWarp;
 // Registers a thread: 72 at launch, 4 * 80 + 2 * 64 + 56 = 7 * 72 afterwards.
 constexpr int kSoftmaxRegs = 80, kConvertRegs = 64, kOtherRegs = 56;
 constexpr int kHalfTokens = kTileTokens / 2;  // of a softmax thread
-constexpr float kMostWeight = 8192.0f;
 constexpr uint32_t kMinusInf = 0xff800000u;
 
 // One row tile of queries, or one tile of K or V: panels of 64 channels, 128

@@ -117,26 +117,28 @@ def _device_ok(index):
 
 def require_device(*tensors):
     """All tensors on one CUDA device of compute capability 10.x (B200 class)."""
-    dev = None
+    index, first = -1, None
     for t in tensors:
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise ValueError("Inputs must be CUDA tensors on a B200 (sm_100) device")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+        if first is None:
+            index, first = t.get_device(), t
+        elif t.get_device() != index:
             raise ValueError("Inputs must share one CUDA device")
-    if dev is None:
+    if first is None:
         raise ValueError("No CUDA tensor given")
-    if not _device_ok(dev.index):
+    if not _device_ok(index):
         raise ValueError("These kernels target sm_100 (B200); got compute capability "
-                         + ".".join(map(str, torch.cuda.get_device_capability(dev.index))))
-    return dev
+                         + ".".join(map(str, torch.cuda.get_device_capability(index))))
+    return first.device
 
 
 def stream_ptr(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream's cudaStream_t (the raw handle: torch.cuda.current_stream
+    builds a Stream object for it, 3 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def check(status, what):

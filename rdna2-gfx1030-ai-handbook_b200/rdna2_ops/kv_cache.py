@@ -21,6 +21,7 @@ call appends to must belong to one sequence only.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -43,6 +44,11 @@ def _rows(x):
     if x.stride(2) != 1 or x.stride(0) % step or x.stride(1) % step or x.data_ptr() % 16:
         return x.clone(memory_format=torch.contiguous_format)
     return x
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*shape):
+    return nat.library().b2_kv_attention_workspace_bytes(*shape)
 
 
 class PagedKVCache:
@@ -83,29 +89,36 @@ class PagedKVCache:
         self.code = "int8" if k_codes.dtype == torch.int8 else "e4m3"
         self._workspaces = {}  # one for each stream: calls on one stream follow each other
 
+    def _memory(self):
+        """The codes and scales as the C entry points take them."""
+        return (self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+                self.num_pages)
+
     # ------------------------------------------------------------- arguments
     def _call(self, x, name, lengths, table, offsets):
         """Checks a call's packed tokens and its paging; returns (device, tokens, batch, width)."""
         if not isinstance(x, torch.Tensor) or x.dtype not in _args.FLOAT_DTYPES:
             raise TypeError(f"{name} must be an fp32, fp16 or bf16 tensor")
-        if x.ndim != 3 or x.shape[2] != self.head_dim:
-            raise ValueError(f"{name} must be [tokens, heads, {self.head_dim}], got {tuple(x.shape)}")
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != self.head_dim:
+            raise ValueError(f"{name} must be [tokens, heads, {self.head_dim}], got {tuple(shape)}")
         dev = nat.require_device(self.k_codes, x, lengths, table, offsets)
         if lengths.dtype != torch.int32 or table.dtype != torch.int32 or (
                 offsets is not None and offsets.dtype != torch.int32):
             raise TypeError("lengths, table and offsets must be int32")
-        if lengths.ndim != 1 or table.ndim != 2 or table.shape[0] != lengths.shape[0]:
+        paging = table.shape
+        if lengths.ndim != 1 or len(paging) != 2 or paging[0] != lengths.shape[0]:
             raise ValueError(f"lengths must be [batch] and table [batch, pages], got {tuple(lengths.shape)} "
-                             f"and {tuple(table.shape)}")
+                             f"and {tuple(paging)}")
         if not (lengths.is_contiguous() and table.is_contiguous()):
             raise ValueError("lengths and table must be contiguous")
-        tokens, batch = x.shape[0], lengths.shape[0]
+        tokens, (batch, width) = shape[0], paging
         if offsets is None:
             if batch == 0 and tokens or batch and tokens % batch:
                 raise ValueError(f"{tokens} tokens do not divide among {batch} sequences; pass offsets")
         elif offsets.shape != (batch + 1,) or not offsets.is_contiguous():
             raise ValueError(f"offsets must be contiguous [{batch + 1}], got {tuple(offsets.shape)}")
-        return dev, tokens, batch, table.shape[1]
+        return dev, tokens, batch, width
 
     # ---------------------------------------------------------------- append
     def append(self, k, v, lengths, table, *, offsets=None, q=None, angles=None, layout="half"):
@@ -151,8 +164,7 @@ class PagedKVCache:
             k.stride(1), v.stride(0), v.stride(1), lengths.data_ptr(), nat.ptr(offsets), batch, table.data_ptr(), width,
             nat.ptr(q), 0 if q is None else q.shape[1], 0 if q is None else q.stride(0),
             0 if q is None else q.stride(1), nat.ptr(rotated), nat.ptr(angles), rows, rotary_dim, LAYOUTS[layout],
-            _CODE_INDEX[self.k_codes.dtype], self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scale.data_ptr(),
-            self.v_scale.data_ptr(), self.num_pages, self.page_size, nat.stream_ptr(dev)), "b2_kv_append")
+            _CODE_INDEX[self.k_codes.dtype], *self._memory(), self.page_size, nat.stream_ptr(dev)), "b2_kv_append")
         return rotated
 
     # ---------------------------------------------------------------- attend
@@ -192,16 +204,14 @@ class PagedKVCache:
         if tokens:
             q = _rows(q)
             lib, stream = nat.library(), nat.stream_ptr(dev)
-            need = lib.b2_kv_attention_workspace_bytes(tokens, batch, max_new, heads, self.kv_heads, self.head_dim,
-                                                       width, self.page_size)
+            need = _workspace_bytes(tokens, batch, max_new, heads, self.kv_heads, self.head_dim, width, self.page_size)
             work = self._workspaces.get(stream)
             if work is None or work.numel() < need:
                 work = self._workspaces[stream] = torch.zeros(need, device=dev, dtype=torch.uint8)
             nat.check(lib.b2_kv_attention(
                 q.data_ptr(), nat.DTYPE_CODE[q.dtype], tokens, heads, q.stride(0), q.stride(1), lengths.data_ptr(),
                 nat.ptr(offsets), batch, max_new, table.data_ptr(), width, _CODE_INDEX[self.k_codes.dtype],
-                self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
-                self.num_pages, self.kv_heads, self.page_size, self.head_dim, scale, int(causal), window or 0,
+                *self._memory(), self.kv_heads, self.page_size, self.head_dim, scale, int(causal), window or 0,
                 out.data_ptr(), nat.ptr(lse), work.data_ptr(), work.numel(), stream), "b2_kv_attention")
         return (out, lse) if return_lse else out
 
@@ -219,11 +229,10 @@ class PagedKVCache:
             raise ValueError(f"pages must be contiguous [n], got {tuple(pages.shape)}")
         nat.eager_only()
         shape = (pages.shape[0], self.kv_heads, self.page_size, self.head_dim)
-        k, v = torch.empty((2, *shape), device=dev, dtype=dtype).unbind()
+        k, v = torch.empty(shape, device=dev, dtype=dtype), torch.empty(shape, device=dev, dtype=dtype)
         scales = torch.empty((2, *shape[:2]), device=dev, dtype=torch.float32) if return_scales else None
         nat.check(nat.library().b2_kv_read(
-            self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
-            _CODE_INDEX[self.k_codes.dtype], self.num_pages, self.kv_heads, self.page_size, self.head_dim,
-            pages.data_ptr(), shape[0], nat.DTYPE_CODE[dtype], k.data_ptr(), v.data_ptr(), nat.ptr(scales),
+            *self._memory()[:4], _CODE_INDEX[self.k_codes.dtype], self.num_pages, self.kv_heads, self.page_size,
+            self.head_dim, pages.data_ptr(), shape[0], nat.DTYPE_CODE[dtype], k.data_ptr(), v.data_ptr(), nat.ptr(scales),
             nat.stream_ptr(dev)), "b2_kv_read")
-        return (k, v, scales[0], scales[1]) if return_scales else (k, v)
+        return (k, v, *scales.unbind()) if return_scales else (k, v)
