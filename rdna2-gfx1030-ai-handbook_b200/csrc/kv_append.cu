@@ -39,11 +39,15 @@ struct AppendParams {
   void* q_out;
   int64_t q_token, q_head;
   int q_heads;
-  int64_t slots;   // blocks of tokens this call may touch, at most
-  int64_t kv_ctas; // slots * kv_heads * 2, the rest of the grid rotates queries
+  int64_t slots;    // blocks of tokens this call may touch, at most
+  int slots_each;   // of every sequence, where all have the same number of tokens, else 0
+  int64_t kv_ctas;  // for slots * kv_heads * 2 blocks; the rest of the grid rotates queries
 };
 
 constexpr int kAppendThreads = 256;
+// Rows of a block that a thread keeps, rotated and in fp32, between finding
+// the block's largest value and quantizing.
+constexpr int kHold = 2;
 
 // Slot s of the call belongs to the sequence with first_slot(b) <= s; the
 // slots of a sequence are enough for the blocks that its tokens touch,
@@ -52,21 +56,40 @@ __device__ __forceinline__ int64_t first_slot(const Tokens& tok, int b, int page
   return static_cast<int64_t>(tok.begin(b)) / page + 2 * static_cast<int64_t>(b);
 }
 
-template <typename T, int DIM, int CODE>
-__device__ __forceinline__ void append_block(const AppendParams& p, int64_t item) {
+// The larger one, or NaN where either is (fmaxf drops it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// One block of one head, keys or values, by THREADS threads: a warp of its
+// own where sequences bring a few tokens each, a CTA where they bring pages
+// of them.  Rows beyond the kHold that a thread keeps are read, from the
+// second-level cache as a rule, and rotated again.
+template <typename T, int DIM, int CODE, int THREADS>
+__device__ __forceinline__ void append_block(const AppendParams& p, int64_t item, int tid) {
   constexpr int V = Vec<T>::kN;
   constexpr int kLanes = DIM / (2 * V);  // lanes a token
-  constexpr int kRows = kAppendThreads / kLanes;
+  constexpr int kRows = THREADS / kLanes;
   const bool is_v = item & 1;
   const int head = static_cast<int>((item >> 1) % p.kv_heads);
   const int64_t slot = (item >> 1) / p.kv_heads;
 
-  const int b = warp_search(p.tok.batch, slot, [&](int i) { return first_slot(p.tok, i, p.page); });
+  int b;
+  int64_t nth;  // block of the sequence's tokens, counted from the first that the call touches
+  if (p.slots_each) {
+    b = static_cast<int>(slot / p.slots_each);
+    nth = slot % p.slots_each;
+  } else {
+    b = warp_search(p.tok.batch, slot, [&](int i) { return first_slot(p.tok, i, p.page); });
+    nth = slot - first_slot(p.tok, b, p.page);
+  }
   const int first = p.tok.begin(b);
   const int count = p.tok.begin(b + 1) - first;
   const int64_t start = static_cast<int64_t>(__ldg(p.tok.lengths + b)) - count;  // position of the first new token
   // block index of this slot, and the positions [from, to) that it receives
-  const int64_t block = (start > 0 ? start : 0) / p.page + (slot - first_slot(p.tok, b, p.page));
+  const int64_t block = (start > 0 ? start : 0) / p.page + nth;
   int64_t from = block * p.page, to = from + p.page;
   const bool earlier = from < start;
   from = from > start ? from : start;
@@ -74,83 +97,118 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int64_t item
   to = to < start + count ? to : start + count;
   if (from >= to || block >= p.width) return;
   const int64_t page_id = __ldg(p.table + static_cast<int64_t>(b) * p.width + block);
-  if (page_id < 0 || page_id >= p.pages) return;
 
-  const int u = threadIdx.x % kLanes, row0 = threadIdx.x / kLanes;
-  const RotaryUnit unit = rotary_unit<V>(u, is_v ? 0 : p.rot, p.interleaved);
-  const T* x = static_cast<const T*>(is_v ? p.v : p.k) + head * (is_v ? p.v_head : p.k_head);
+  // this thread's rows of the block's new ones, kRows apart
+  const int rows = static_cast<int>(to - from), row0 = tid / kLanes;
+  const RotaryUnit unit = rotary_unit<V>(tid % kLanes, is_v ? 0 : p.rot, p.interleaved);
   const int64_t x_token = is_v ? p.v_token : p.k_token;
-  uint8_t* codes = (is_v ? p.v_codes : p.k_codes) + (page_id * p.kv_heads + head) * p.page * DIM;
-  float* scale = (is_v ? p.v_scale : p.k_scale) + page_id * p.kv_heads + head;
-
-  const auto load = [&](int64_t position, float (&a)[V], float (&c)[V]) {
-    const T* row = x + (first + (position - start)) * x_token;
-    Vec<T>::unpack(ldg_v4(row + unit.o0), a);
-    Vec<T>::unpack(ldg_v4(row + unit.o1), c);
-    if (unit.pair >= 0) {
-      float cos[V], sin[V];
-      load_angles<V>(p.angles, p.rows, p.rot, position, unit.pair, cos, sin);
-      rotate_unit<V>(a, c, cos, sin, p.interleaved);
+  const T* x = static_cast<const T*>(is_v ? p.v : p.k) + head * (is_v ? p.v_head : p.k_head) +
+               (first + (from - start) + row0) * x_token;
+  const float* angles = p.angles + (from + row0) * p.rot + unit.pair;
+  const int in_table = to <= p.rows ? rows : static_cast<int>(p.rows > from ? p.rows - from : 0);
+  float a[kHold][V], c[kHold][V];
+  const auto load = [&](int batch) {
+    uint4 va[kHold], vb[kHold];
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) {
+      const int row = (batch * kHold + i) * kRows;
+      va[i] = vb[i] = make_uint4(0, 0, 0, 0);
+      if (row0 + row < rows) {
+        va[i] = ldg_v4(x + row * x_token + unit.o0);
+        vb[i] = ldg_v4(x + row * x_token + unit.o1);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) {
+      const int row = (batch * kHold + i) * kRows;
+      Vec<T>::unpack(va[i], a[i]);
+      Vec<T>::unpack(vb[i], c[i]);
+      if (unit.pair >= 0 && row0 + row < rows) {
+        float cos[V], sin[V];
+        if (row0 + row < in_table) {
+          load_angles<V>(angles + row * p.rot, p.rot, cos, sin);
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) cos[j] = sin[j] = __int_as_float(0x7fffffff);
+        }
+        rotate_unit<V>(a[i], c[i], cos, sin, p.interleaved);
+      }
     }
   };
 
-  // largest magnitude as ordered bits: an infinity or a NaN stays on top
-  uint32_t top = 0;
-  for (int64_t pos = from + row0; pos < to; pos += kRows) {
-    float a[V], c[V];
-    load(pos, a, c);
+  // the largest magnitude; a NaN stays, and rows that are not there are zero
+  float most = 0.0f;
+  const int batches = (rows + kRows * kHold - 1) / (kRows * kHold);
+#pragma unroll 1
+  for (int batch = 0; batch < batches; ++batch) {
+    load(batch);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      top = max(top, __float_as_uint(a[i]) & 0x7fffffffu);
-      top = max(top, __float_as_uint(c[i]) & 0x7fffffffu);
-    }
+    for (int i = 0; i < kHold; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) most = max_nan(most, max_nan(fabsf(a[i][j]), fabsf(c[i][j])));
   }
-  __shared__ uint32_t tops[kAppendThreads / kWarp];
-  top = __reduce_max_sync(kFullMask, top);
-  if (threadIdx.x % kWarp == 0) tops[threadIdx.x / kWarp] = top;
+  uint32_t top = __float_as_uint(most) & 0x7fffffffu;  // ordered like the numbers, NaN above them
+  if (page_id < 0 || page_id >= p.pages) return;
+  uint8_t* codes = (is_v ? p.v_codes : p.k_codes) + (page_id * p.kv_heads + head) * p.page * DIM;
+  float* scale = (is_v ? p.v_scale : p.k_scale) + page_id * p.kv_heads + head;
+  const int slot0 = static_cast<int>(from - block * p.page);  // place of the first new row
   const float was = earlier ? *scale : 0.0f;
-  __syncthreads();
+  top = __reduce_max_sync(kFullMask, top);
+  if constexpr (THREADS > kWarp) {
+    __shared__ uint32_t tops[THREADS / kWarp];
+    if (tid % kWarp == 0) tops[tid / kWarp] = top;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kAppendThreads / kWarp; ++i) top = max(top, tops[i]);
+    for (int i = 0; i < THREADS / kWarp; ++i) top = max(top, tops[i]);
+  } else {
+    __syncwarp();  // every lane has read the scale
+  }
   float now = __fdiv_rn(__uint_as_float(top), CODE == kCodeInt8 ? 127.0f : 448.0f);
   now = now < kScaleFloor ? kScaleFloor : now;
   now = (was > now || was != was) ? was : now;
 
   if (earlier && now != was) {
     const float ratio = __fdiv_rn(was, now);
-    const int words = static_cast<int>(from - block * p.page) * (DIM / 4);
-    for (int i = threadIdx.x; i < words; i += kAppendThreads) {
-      const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[i];
-      uint32_t n = 0;
+    const int words = slot0 * (DIM / 4);
+    uint32_t* row = reinterpret_cast<uint32_t*>(codes);
+    for (int i = tid; i < words; i += THREADS) {
+      const uint32_t w = row[i];
+      float f[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        n |= to_code<CODE>(__fmul_rn(from_code<CODE>((w >> (8 * j)) & 0xffu), ratio)) << (8 * j);
-      reinterpret_cast<uint32_t*>(codes)[i] = n;
+      for (int j = 0; j < 4; ++j) f[j] = __fmul_rn(from_code<CODE>((w >> (8 * j)) & 0xffu), ratio);
+      row[i] = pack_codes<CODE>(f, now);
     }
   }
-  if (threadIdx.x == 0) *scale = now;
+  if (tid == 0) *scale = now;
 
   const float inv = __fdiv_rn(1.0f, now);
-  for (int64_t pos = from + row0; pos < to; pos += kRows) {
-    float a[V], c[V];
-    load(pos, a, c);
-    uint8_t* row = codes + (pos - block * p.page) * DIM;
-    uint32_t wa[V / 4], wc[V / 4];
+#pragma unroll 1
+  for (int batch = batches - 1; batch >= 0; --batch) {
+    if (batch != batches - 1) load(batch);
 #pragma unroll
-    for (int i = 0; i < V / 4; ++i) {
-      wa[i] = wc[i] = 0;
+    for (int i = 0; i < kHold; ++i) {
+      const int row = row0 + (batch * kHold + i) * kRows;
+      if (row >= rows) break;
+      uint32_t wa[V / 4], wc[V / 4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        wa[i] |= to_code<CODE>(__fmul_rn(a[4 * i + j], inv)) << (8 * j);
-        wc[i] |= to_code<CODE>(__fmul_rn(c[4 * i + j], inv)) << (8 * j);
+      for (int j = 0; j < V / 4; ++j) {
+        float f[4], g[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          f[k] = __fmul_rn(a[i][4 * j + k], inv);
+          g[k] = __fmul_rn(c[i][4 * j + k], inv);
+        }
+        wa[j] = pack_codes<CODE>(f, now);
+        wc[j] = pack_codes<CODE>(g, now);
       }
-    }
-    if constexpr (V == 8) {
-      *reinterpret_cast<uint2*>(row + unit.o0) = make_uint2(wa[0], wa[1]);
-      *reinterpret_cast<uint2*>(row + unit.o1) = make_uint2(wc[0], wc[1]);
-    } else {
-      *reinterpret_cast<uint32_t*>(row + unit.o0) = wa[0];
-      *reinterpret_cast<uint32_t*>(row + unit.o1) = wc[0];
+      uint8_t* out = codes + (slot0 + row) * DIM;
+      if constexpr (V == 8) {
+        *reinterpret_cast<uint2*>(out + unit.o0) = make_uint2(wa[0], wa[1]);
+        *reinterpret_cast<uint2*>(out + unit.o1) = make_uint2(wc[0], wc[1]);
+      } else {
+        *reinterpret_cast<uint32_t*>(out + unit.o0) = wa[0];
+        *reinterpret_cast<uint32_t*>(out + unit.o1) = wc[0];
+      }
     }
   }
 }
@@ -203,25 +261,41 @@ __device__ __forceinline__ void rotate_queries(const AppendParams& p, int64_t wa
   }
 }
 
-template <typename T, int DIM, int CODE>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendParams p) {
+template <typename T, int DIM, int CODE, int THREADS>
+__global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(AppendParams p) {
   const int64_t cta = blockIdx.x;
   if (cta < p.kv_ctas) {
-    append_block<T, DIM, CODE>(p, cta);
+    const int64_t item = cta * (kAppendThreads / THREADS) + threadIdx.x / THREADS;
+    if (item < p.slots * p.kv_heads * 2) append_block<T, DIM, CODE, THREADS>(p, item, threadIdx.x % THREADS);
   } else {
     rotate_queries<T, DIM>(p, (cta - p.kv_ctas) * (kAppendThreads / kWarp) + threadIdx.x / kWarp);
   }
 }
 
+// Up to this many tokens a sequence (on the average, where they differ) a
+// block is a warp's: most CTAs would idle otherwise.
+constexpr int64_t kFewTokens = 4;
+
 template <typename T, int DIM, int CODE>
 cudaError_t run_append(AppendParams p, cudaStream_t stream) {
   constexpr int kHeads = kWarp / (DIM / (2 * Vec<T>::kN));
-  p.slots = static_cast<int64_t>(p.tok.tokens) / p.page + 2 * static_cast<int64_t>(p.tok.batch);
-  p.kv_ctas = p.slots * p.kv_heads * 2;
+  const bool few = p.tok.tokens <= kFewTokens * p.tok.batch;
+  if (p.tok.offsets == nullptr) {
+    p.slots_each = p.tok.each == 1 ? 1 : (p.tok.each - 2) / p.page + 2;
+    p.slots = static_cast<int64_t>(p.slots_each) * p.tok.batch;
+  } else {
+    p.slots = static_cast<int64_t>(p.tok.tokens) / p.page + 2 * static_cast<int64_t>(p.tok.batch);
+  }
+  const int64_t blocks = p.slots * p.kv_heads * 2;
+  p.kv_ctas = few ? ceil_div64(blocks, kAppendThreads / kWarp) : blocks;
   const int64_t chunks = p.q != nullptr ? ceil_div64(p.q_heads, kHeads * kQUnroll) : 0;
   const int64_t grid = p.kv_ctas + ceil_div64(chunks * p.tok.tokens, kAppendThreads / kWarp);
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
-  append_kernel<T, DIM, CODE><<<static_cast<unsigned>(grid), kAppendThreads, 0, stream>>>(p);
+  if (few) {
+    append_kernel<T, DIM, CODE, kWarp><<<static_cast<unsigned>(grid), kAppendThreads, 0, stream>>>(p);
+  } else {
+    append_kernel<T, DIM, CODE, kAppendThreads><<<static_cast<unsigned>(grid), kAppendThreads, 0, stream>>>(p);
+  }
   return cudaGetLastError();
 }
 

@@ -87,6 +87,31 @@ struct Vec<__nv_bfloat16> {
 __device__ __forceinline__ uint4 ldg_v4(const void* p) { return __ldg(static_cast<const uint4*>(p)); }
 
 // ------------------------------------------------------------------- rotation
+// Two fp32 numbers in a register pair.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void unpair(uint64_t d, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // (a, b) -> (a cos - b sin, b cos + a sin), products and sums each rounded to
 // fp32 (no contraction), so the result is the same as elementwise torch.
 __device__ __forceinline__ void rotate_pair(float& a, float& b, float cos, float sin) {
@@ -131,7 +156,23 @@ __device__ __forceinline__ void rotate_unit(float (&a)[V], float (&b)[V], const 
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) rotate_pair(a[i], b[i], cos[i], sin[i]);
+    for (int i = 0; i < V; i += 2) {  // rotate_pair for two pairs at once: b (-sin) is -(b sin)
+      const uint64_t x = pair_of(a[i], a[i + 1]), y = pair_of(b[i], b[i + 1]);
+      const uint64_t c = pair_of(cos[i], cos[i + 1]), s = pair_of(sin[i], sin[i + 1]);
+      unpair(add_pair(mul_pair(x, c), mul_pair(y, pair_of(-sin[i], -sin[i + 1]))), a[i], a[i + 1]);
+      unpair(add_pair(mul_pair(y, c), mul_pair(x, s)), b[i], b[i + 1]);
+    }
+  }
+}
+
+template <int V>
+__device__ __forceinline__ void load_angles(const float* row, int rot, float (&cos)[V], float (&sin)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; i += 4) {
+    const float4 x = __ldg(reinterpret_cast<const float4*>(row + i));
+    const float4 y = __ldg(reinterpret_cast<const float4*>(row + rot / 2 + i));
+    cos[i] = x.x, cos[i + 1] = x.y, cos[i + 2] = x.z, cos[i + 3] = x.w;
+    sin[i] = y.x, sin[i + 1] = y.y, sin[i + 2] = y.z, sin[i + 3] = y.w;
   }
 }
 
@@ -145,14 +186,7 @@ __device__ __forceinline__ void load_angles(const float* angles, int64_t rows, i
     for (int i = 0; i < V; ++i) cos[i] = sin[i] = __int_as_float(0x7fffffff);
     return;
   }
-  const float* c = angles + position * rot + pair;
-#pragma unroll
-  for (int i = 0; i < V; i += 4) {
-    const float4 x = __ldg(reinterpret_cast<const float4*>(c + i));
-    const float4 y = __ldg(reinterpret_cast<const float4*>(c + rot / 2 + i));
-    cos[i] = x.x, cos[i + 1] = x.y, cos[i + 2] = x.z, cos[i + 3] = x.w;
-    sin[i] = y.x, sin[i + 1] = y.y, sin[i + 2] = y.z, sin[i + 3] = y.w;
-  }
+  load_angles<V>(angles + position * rot + pair, rot, cos, sin);
 }
 
 // --------------------------------------------------------- tokens of a call
@@ -218,15 +252,24 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t
   }
 }
 
-// fp32 -> one code, round to nearest even, saturating; no code is NaN (a NaN
-// shows by its block's scale).
+// Four codes of numbers x / scale, round to nearest even.  They are in the
+// codes' range but for a rounding, since the scale covers the block (adding
+// 1.5 * 2^23 leaves the integer in the low byte; e4m3 saturates).  Where the
+// scale is no number the codes are 0: a NaN or an infinity shows by the scale.
 template <int CODE>
-__device__ __forceinline__ uint32_t to_code(float x) {
+__device__ __forceinline__ uint32_t pack_codes(const float (&x)[4], float scale) {
+  uint32_t w;
   if constexpr (CODE == kCodeInt8) {
-    return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(x, -127.0f), 127.0f))) & 0xffu;
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(__fadd_rn(x[i], 12582912.0f));
+    w = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
   } else {
-    return __nv_cvt_float_to_fp8(fminf(fmaxf(x, -448.0f), 448.0f), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+    w = lo | hi << 16;
   }
+  return scale < INFINITY ? w : 0u;
 }
 
 template <int CODE>
