@@ -31,7 +31,7 @@ struct AppendParams {
   float* k_scale;
   float* v_scale;
   int64_t pages;
-  int page, kv_heads;
+  int page, page_shift, kv_heads;
   const float* angles;
   int64_t rows;
   int rot, interleaved;
@@ -39,9 +39,9 @@ struct AppendParams {
   void* q_out;
   int64_t q_token, q_head;
   int q_heads;
-  int64_t slots;    // blocks of tokens this call may touch, at most
+  int slots;        // blocks of tokens this call may touch, at most
   int slots_each;   // of every sequence, where all have the same number of tokens, else 0
-  int64_t kv_ctas;  // for slots * kv_heads * 2 blocks; the rest of the grid rotates queries
+  int kv_ctas;      // for slots * kv_heads * 2 blocks; the rest of the grid rotates queries
 };
 
 constexpr int kAppendThreads = 256;
@@ -52,8 +52,8 @@ constexpr int kHold = 2;
 // Slot s of the call belongs to the sequence with first_slot(b) <= s; the
 // slots of a sequence are enough for the blocks that its tokens touch,
 // floor((n - 2) / page) + 2 at most.
-__device__ __forceinline__ int64_t first_slot(const Tokens& tok, int b, int page) {
-  return static_cast<int64_t>(tok.begin(b)) / page + 2 * static_cast<int64_t>(b);
+__device__ __forceinline__ int first_slot(const Tokens& tok, int b, int page_shift) {
+  return (tok.begin(b) >> page_shift) + 2 * b;
 }
 
 // The larger one, or NaN where either is (fmaxf drops it).
@@ -68,29 +68,28 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // of them.  Rows beyond the kHold that a thread keeps are read, from the
 // second-level cache as a rule, and rotated again.
 template <typename T, int DIM, int CODE, int THREADS>
-__device__ __forceinline__ void append_block(const AppendParams& p, int64_t item, int tid) {
+__device__ __forceinline__ void append_block(const AppendParams& p, uint32_t item, int tid) {
   constexpr int V = Vec<T>::kN;
   constexpr int kLanes = DIM / (2 * V);  // lanes a token
   constexpr int kRows = THREADS / kLanes;
   const bool is_v = item & 1;
-  const int head = static_cast<int>((item >> 1) % p.kv_heads);
-  const int64_t slot = (item >> 1) / p.kv_heads;
+  const int slot = static_cast<int>((item >> 1) / static_cast<uint32_t>(p.kv_heads));
+  const int head = static_cast<int>((item >> 1) - slot * static_cast<uint32_t>(p.kv_heads));
 
-  int b;
-  int64_t nth;  // block of the sequence's tokens, counted from the first that the call touches
+  int b, nth;  // block of the sequence's tokens, counted from the first that the call touches
   if (p.slots_each) {
-    b = static_cast<int>(slot / p.slots_each);
-    nth = slot % p.slots_each;
+    b = slot / p.slots_each;
+    nth = slot - b * p.slots_each;
   } else {
-    b = warp_search(p.tok.batch, slot, [&](int i) { return first_slot(p.tok, i, p.page); });
-    nth = slot - first_slot(p.tok, b, p.page);
+    b = warp_search(p.tok.batch, slot, [&](int i) { return first_slot(p.tok, i, p.page_shift); });
+    nth = slot - first_slot(p.tok, b, p.page_shift);
   }
   const int first = p.tok.begin(b);
   const int count = p.tok.begin(b + 1) - first;
   const int64_t start = static_cast<int64_t>(__ldg(p.tok.lengths + b)) - count;  // position of the first new token
   // block index of this slot, and the positions [from, to) that it receives
-  const int64_t block = (start > 0 ? start : 0) / p.page + nth;
-  int64_t from = block * p.page, to = from + p.page;
+  const int64_t block = ((start > 0 ? start : 0) >> p.page_shift) + nth;
+  int64_t from = block << p.page_shift, to = from + p.page;
   const bool earlier = from < start;
   from = from > start ? from : start;
   from = from > 0 ? from : 0;
@@ -151,7 +150,7 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int64_t item
   if (page_id < 0 || page_id >= p.pages) return;
   uint8_t* codes = (is_v ? p.v_codes : p.k_codes) + (page_id * p.kv_heads + head) * p.page * DIM;
   float* scale = (is_v ? p.v_scale : p.k_scale) + page_id * p.kv_heads + head;
-  const int slot0 = static_cast<int>(from - block * p.page);  // place of the first new row
+  const int slot0 = static_cast<int>(from - (block << p.page_shift));  // place of the first new row
   const float was = earlier ? *scale : 0.0f;
   top = __reduce_max_sync(kFullMask, top);
   if constexpr (THREADS > kWarp) {
@@ -217,15 +216,14 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int64_t item
 constexpr int kQUnroll = 4;
 
 template <typename T, int DIM>
-__device__ __forceinline__ void rotate_queries(const AppendParams& p, int64_t warp) {
+__device__ __forceinline__ void rotate_queries(const AppendParams& p, uint32_t warp) {
   constexpr int V = Vec<T>::kN;
   constexpr int kLanes = DIM / (2 * V), kHeads = kWarp / kLanes;
-  const int chunks = (p.q_heads + kHeads * kQUnroll - 1) / (kHeads * kQUnroll);
-  const int64_t token = warp / chunks;
+  const uint32_t chunks = (p.q_heads + kHeads * kQUnroll - 1) / (kHeads * kQUnroll);
+  const int token = static_cast<int>(warp / chunks);
   if (token >= p.tok.tokens) return;
-  const int b = p.tok.offsets == nullptr
-                    ? static_cast<int>(token) / p.tok.each
-                    : warp_search(p.tok.batch, token, [&](int i) { return static_cast<int64_t>(p.tok.begin(i)); });
+  const int b = p.tok.offsets == nullptr ? token / p.tok.each
+                                         : warp_search(p.tok.batch, token, [&](int i) { return p.tok.begin(i); });
   const int64_t position = static_cast<int64_t>(__ldg(p.tok.lengths + b)) - p.tok.begin(b + 1) + token;
   const int lane = threadIdx.x % kWarp;
   const RotaryUnit unit = rotary_unit<V>(lane % kLanes, p.rot, p.interleaved);
@@ -233,7 +231,7 @@ __device__ __forceinline__ void rotate_queries(const AppendParams& p, int64_t wa
   if (unit.pair >= 0) load_angles<V>(p.angles, p.rows, p.rot, position, unit.pair, cos, sin);
   const int head0 = static_cast<int>(warp % chunks) * kHeads * kQUnroll + lane / kLanes;
   const T* x = static_cast<const T*>(p.q) + token * p.q_token;
-  T* out = static_cast<T*>(p.q_out) + token * p.q_heads * DIM;
+  T* out = static_cast<T*>(p.q_out) + static_cast<int64_t>(token) * p.q_heads * DIM;
   uint4 va[kQUnroll], vb[kQUnroll];
 #pragma unroll
   for (int i = 0; i < kQUnroll; ++i) {
@@ -263,12 +261,14 @@ __device__ __forceinline__ void rotate_queries(const AppendParams& p, int64_t wa
 
 template <typename T, int DIM, int CODE, int THREADS>
 __global__ void __launch_bounds__(kAppendThreads, 3) append_kernel(AppendParams p) {
-  const int64_t cta = blockIdx.x;
+  const int cta = blockIdx.x;
   if (cta < p.kv_ctas) {
-    const int64_t item = cta * (kAppendThreads / THREADS) + threadIdx.x / THREADS;
-    if (item < p.slots * p.kv_heads * 2) append_block<T, DIM, CODE, THREADS>(p, item, threadIdx.x % THREADS);
+    const uint32_t item = static_cast<uint32_t>(cta) * (kAppendThreads / THREADS) + threadIdx.x / THREADS;
+    if (item < static_cast<uint32_t>(p.slots) * p.kv_heads * 2)
+      append_block<T, DIM, CODE, THREADS>(p, item, threadIdx.x % THREADS);
   } else {
-    rotate_queries<T, DIM>(p, (cta - p.kv_ctas) * (kAppendThreads / kWarp) + threadIdx.x / kWarp);
+    constexpr int kWarps = kAppendThreads / kWarp;
+    rotate_queries<T, DIM>(p, static_cast<uint32_t>(cta - p.kv_ctas) * kWarps + threadIdx.x / kWarp);
   }
 }
 
@@ -282,13 +282,14 @@ cudaError_t run_append(AppendParams p, cudaStream_t stream) {
   const bool few = p.tok.tokens <= kFewTokens * p.tok.batch;
   if (p.tok.offsets == nullptr) {
     p.slots_each = p.tok.each == 1 ? 1 : (p.tok.each - 2) / p.page + 2;
-    p.slots = static_cast<int64_t>(p.slots_each) * p.tok.batch;
+    p.slots = p.slots_each * p.tok.batch;  // at most 2 * tokens
   } else {
-    p.slots = static_cast<int64_t>(p.tok.tokens) / p.page + 2 * static_cast<int64_t>(p.tok.batch);
+    p.slots = (p.tok.tokens >> p.page_shift) + 2 * p.tok.batch;
   }
-  const int64_t blocks = p.slots * p.kv_heads * 2;
-  p.kv_ctas = few ? ceil_div64(blocks, kAppendThreads / kWarp) : blocks;
+  const int64_t blocks = static_cast<int64_t>(p.slots) * p.kv_heads * 2;
   const int64_t chunks = p.q != nullptr ? ceil_div64(p.q_heads, kHeads * kQUnroll) : 0;
+  if (blocks > INT32_MAX || chunks * p.tok.tokens > INT32_MAX) return cudaErrorInvalidValue;
+  p.kv_ctas = static_cast<int>(few ? ceil_div64(blocks, kAppendThreads / kWarp) : blocks);
   const int64_t grid = p.kv_ctas + ceil_div64(chunks * p.tok.tokens, kAppendThreads / kWarp);
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
   if (few) {
@@ -316,10 +317,10 @@ __global__ void __launch_bounds__(256) read_kernel(const uint8_t* k_codes, const
                                                    const float* v_scale, const int32_t* pages, int64_t n,
                                                    int64_t num_pages, int kv_heads, int block_bytes, T* k_out, T* v_out,
                                                    float* scales_out) {
-  const int64_t item = blockIdx.x;  // (page, head, K or V)
+  const uint32_t item = blockIdx.x;  // (page, head, K or V)
   const bool is_v = item & 1;
-  const int head = static_cast<int>((item >> 1) % kv_heads);
-  const int64_t i = (item >> 1) / kv_heads;
+  const int64_t i = (item >> 1) / static_cast<uint32_t>(kv_heads);
+  const int head = static_cast<int>((item >> 1) - i * kv_heads);
   const int64_t page = pages[i];
   T* out = (is_v ? v_out : k_out) + (i * kv_heads + head) * block_bytes;
   const bool held = page >= 0 && page < num_pages;
@@ -412,6 +413,7 @@ int b2_kv_append(const void* k, const void* v, int dtype, int64_t tokens, int64_
   p.v_scale = v_scale;
   p.pages = pages;
   p.page = static_cast<int>(page);
+  p.page_shift = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
   p.kv_heads = static_cast<int>(kv_heads);
   p.angles = angles;
   p.rows = angle_rows;

@@ -44,18 +44,24 @@ constexpr int kRowsWarps = 8;
 constexpr int kRowsThreads = kRowsWarps * kWarp;
 constexpr int kRowsTile = 16 * kRowsWarps;  // cached tokens a CTA takes at once
 constexpr int kRowsMaxGrid = 1024;
+// What an item costs beside its token tiles, in tiles: the start of its
+// pipeline, its queries and its join.  Shares that left it out made the CTAs
+// with many short sequences the last to finish.
+constexpr int kItemTiles = 4;
 
 // Stages of a warp's ring, 16 tokens of K and V each: two CTAs of an SM with
 // two, or one with four.
 template <int NT>
 constexpr int kStages = NT == 1 ? 2 : 4;
 
-// A run of token tiles of one item: a sequence, a kv head and 8 * NT rows.
+// A run of token tiles (none, if only kItemTiles fall to it) of one item: a sequence, a kv head and 8 * NT rows.
 // Kept in shared memory, the registers being short.
 struct Segment {
   Sequence s;
   int b, head, tile0, take, tiles;
-  int64_t row0, rows, local, at;  // `local` and `at`: its first tile within the sequence's and within all
+  int unit0, units;  // its part of the item's kItemTiles + tiles
+  int row0, rows;
+  int64_t local, at;  // `local` and `at`: its first tile within the sequence's and within all
 };
 
 template <int DIM, int NT>
@@ -113,13 +119,16 @@ __device__ __forceinline__ Segment segment_at(const AttendParams& p, const Seque
   g.b = b;
   g.local = local;
   g.at = at;
-  g.rows = static_cast<int64_t>(s.count) * p.group;
+  g.rows = s.count * p.group;
   g.tiles = rows_tiles(s);
-  const int64_t row_tiles = ceil_div64(g.rows, 8 * NT), item = local / g.tiles;
-  g.tile0 = static_cast<int>(local % g.tiles);
-  g.take = static_cast<int>(min(static_cast<int64_t>(g.tiles - g.tile0), end - at));
-  g.head = static_cast<int>(item / row_tiles);
-  g.row0 = item % row_tiles * (8 * NT);
+  const int row_tiles = (g.rows + 8 * NT - 1) / (8 * NT), all = kItemTiles + g.tiles;
+  const int64_t item = quotient(local, all);
+  g.unit0 = static_cast<int>(local - item * all);
+  g.units = static_cast<int>(min(static_cast<int64_t>(all - g.unit0), end - at));
+  g.tile0 = max(0, g.unit0 - kItemTiles);
+  g.take = max(0, g.unit0 + g.units - kItemTiles) - g.tile0;
+  g.head = static_cast<int>(quotient(item, row_tiles));
+  g.row0 = static_cast<int>(item - static_cast<int64_t>(g.head) * row_tiles) * (8 * NT);
   return g;
 }
 
@@ -142,11 +151,11 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
     fence_mbar_init();
   }
 
-  // ---- this CTA's share of all (item, token tile) pairs, in order
+  // ---- this CTA's share of all items' tiles, in order
   const auto cost = [&](int b) -> int64_t {
     if (b >= p.tok.batch) return 0;
     const Sequence s = load_sequence(p, b);
-    return ceil_div64(static_cast<int64_t>(s.count) * p.group, kRows) * p.kv_heads * rows_tiles(s);
+    return static_cast<int64_t>((s.count * p.group + kRows - 1) / kRows) * p.kv_heads * (kItemTiles + rows_tiles(s));
   };
   // inclusive sum over the CTA's threads, and the sum of all
   const auto scan = [&](int64_t v, int64_t& all) -> int64_t {
@@ -176,7 +185,7 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
   }
   const int64_t parts = min(static_cast<int64_t>(gridDim.x), total);  // CTAs with work: none of them is empty
   if (cta >= parts) return;
-  const int64_t begin = cta * total / parts, end = (cta + 1) * total / parts;
+  const int64_t begin = quotient(cta * total, parts), end = quotient((cta + 1) * total, parts);
   int64_t before = 0;
   for (int base = 0; base < p.tok.batch && before <= begin; base += kRowsThreads) {
     int64_t all = 0, c = first_cost, upto = first_upto;
@@ -242,21 +251,21 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
   start(sh.seg[0]);
   for (int which = 0;; which ^= 1) {
     const Segment& seg = sh.seg[which];
-    const bool more = seg.at + seg.take < end;
+    const bool more = seg.at + seg.units < end;
     if (more && threadIdx.x == kRowsThreads - 1) {  // seen by the others after the barrier below
       Sequence s = seg.s;
       int b = seg.b;
-      int64_t local = seg.local + seg.take;
-      if (local == ceil_div64(seg.rows, kRows) * p.kv_heads * seg.tiles) {
+      int64_t local = seg.local + seg.units;
+      if (local == static_cast<int64_t>((seg.rows + kRows - 1) / kRows) * p.kv_heads * (kItemTiles + seg.tiles)) {
         do {
           s = load_sequence(p, ++b);
         } while (s.count == 0);
         local = 0;
       }
-      sh.seg[which ^ 1] = segment_at<NT>(p, s, b, local, seg.at + seg.take, end);
+      sh.seg[which ^ 1] = segment_at<NT>(p, s, b, local, seg.at + seg.units, end);
     }
     __syncwarp();
-    const int64_t row0 = seg.row0, rows = seg.rows;
+    const int row0 = seg.row0, rows = seg.rows;
     // ---- queries: lane (g, t) holds of row g the channels its key chunks hold
     uint32_t qf[NT][kChunks][8];
     float qa[NT][2], qb[NT][2];  // u = product * qa * ks + qb * ks
@@ -266,7 +275,7 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
     int lo_most = 0, hi_least = INT32_MAX;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int64_t r = row0 + n * 8 + g;
+      const int r = row0 + n * 8 + g;
       uint4 raw_q[kChunks][2];
       uint32_t top = 0;
       float f[kChunks][16], sum = 0.0f;
@@ -315,7 +324,7 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
         qb[n][j] = CODE == kCodeInt8 ? -128.0f * __shfl_sync(kFullMask, sum, 8 * t + 4 * j) * qs : 0.0f;
         m[n][j] = mu[n][j] = -INFINITY;
         l[n][j] = 0.0f;
-        const int64_t rj = row0 + n * 8 + 2 * t + j;
+        const int rj = row0 + n * 8 + 2 * t + j;
         lo[n][j] = 0;
         hi[n][j] = INT32_MAX;  // a row that is not one of the sequence's: whatever it sums is not stored
         if (rj < rows) row_bounds(p, seg.s, seg.s.start + rj / p.group, lo[n][j], hi[n][j]);
@@ -333,6 +342,7 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
     // ---- tokens: each warp its own 16 of every tile
     const int row_a = stage_row<DIM>(g);                                        // key rows row_a, row_a + 8
     const int row_b = stage_row<DIM>(2 * t), row_c = stage_row<DIM>(2 * t + 1);  // value rows, and those + 8
+    const int seg_hi = seg.s.hi;
     for (int i = 0; i < groups; ++i) {
       const int stage = used % kRing, base = base0 + i * kRowsTile;
       if (!__all_sync(kFullMask, mbar_wait(&sh.full[warp][stage], used / kRing & 1, &sh.abort, kSiteProducer,
@@ -344,50 +354,38 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
       const bool here = sh.block[warp][stage] >= 0;
       const float ks = next_ks, vs = next_vs;
       uint4 kw[kChunks][2];
-      uint32_t vw[4][kVWords];
       if (here) {
-        const uint32_t k_at = smem_u32(sh.ring[warp][stage][0]), v_at = smem_u32(sh.ring[warp][stage][1]);
+        const uint32_t k_at = smem_u32(sh.ring[warp][stage][0]);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           const uint32_t at = k_at + stage_byte<DIM>(row_a, (t + 4 * c) * 16);
           kw[c][0] = lds_v4(at);
           kw[c][1] = lds_v4(at + 8 * DIM);
         }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const uint32_t at = v_at + stage_byte<DIM>(x & 1 ? row_c : row_b, g * (DIM / 8)) + (x >> 1) * 8 * DIM;
-          if constexpr (kVWords == 4) {
-            const uint4 w = lds_v4(at);
-            vw[x][0] = w.x, vw[x][1] = w.y, vw[x][2] = w.z, vw[x][3] = w.w;
-          } else {
-            lds_v2(at, vw[x][0], vw[x][1]);
-          }
-        }
-      }
-      __syncwarp();  // the stage has been read
-      if (i + kRing < groups) {
-        issue(i + kRing, next_block);
-        next_block = block_at(seg, i + kRing + 1);
       }
       if (i + 1 < groups) fetch_scales();
-      if (!here) continue;
-      if (base + 16 > seg.s.hi) {  // what lies behind the last token may be no number, and meets weights of zero
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          if (base + (x & 1 ? row_c : row_b) + 8 * (x >> 1) >= seg.s.hi)
-#pragma unroll
-            for (int w = 0; w < kVWords; ++w) vw[x][w] = 0;
+      const auto refill = [&] {  // the stage has been read
+        __syncwarp();
+        if (i + kRing < groups) {
+          issue(i + kRing, next_block);
+          next_block = block_at(seg, i + kRing + 1);
+        }
+      };
+      if (!here) {
+        refill();
+        continue;
       }
       const float lv = value_exponent(vs, 0.0f, largest);
 
-      // scores of tokens row_a and row_a + 8 (rows) for query rows 2t and 2t + 1
-      float sc[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sc[n][j] = 0.0f;
+      // scores of tokens row_a and row_a + 8 (rows) for query rows 2t and
+      // 2t + 1, in a chain of products for each piece of the key row
+      float sc[NT][4], part[kChunks][NT][4];
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) part[c][n][j] = 0.0f;
         const uint32_t w0[4] = {kw[c][0].x, kw[c][0].y, kw[c][0].z, kw[c][0].w};
         const uint32_t w1[4] = {kw[c][1].x, kw[c][1].y, kw[c][1].z, kw[c][1].w};
 #pragma unroll
@@ -396,9 +394,13 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
           to_operand<CODE, true>(w0[k], a[0], a[2]);
           to_operand<CODE, true>(w1[k], a[1], a[3]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(sc[n], a, qf[n][c][2 * k], qf[n][c][2 * k + 1]);
+          for (int n = 0; n < NT; ++n) mma_f16(part[c][n], a, qf[n][c][2 * k], qf[n][c][2 * k + 1]);
         }
       }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[n][j] = kChunks == 1 ? part[0][n][j] : part[0][n][j] + part[kChunks - 1][n][j];
       const bool whole = lo_most <= base && base + 16 <= hi_least;
       // t of the group's tokens, their weights against the references of
       // earlier groups, and whether those have to be raised: a row has none
@@ -458,6 +460,27 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
         pf[n][0] = transpose_8x8(pack_half2(weight[n][0], weight[n][1]));
         pf[n][1] = transpose_8x8(pack_half2(weight[n][2], weight[n][3]));
       }
+      uint32_t vw[4][kVWords];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int row = x & 1 ? row_c : row_b;
+        const uint32_t at =
+            smem_u32(sh.ring[warp][stage][1]) + stage_byte<DIM>(row, g * (DIM / 8)) + (x >> 1) * 8 * DIM;
+        if constexpr (kVWords == 4) {
+          const uint4 w = lds_v4(at);
+          vw[x][0] = w.x, vw[x][1] = w.y, vw[x][2] = w.z, vw[x][3] = w.w;
+        } else {
+          lds_v2(at, vw[x][0], vw[x][1]);
+        }
+      }
+      if (base + 16 > seg_hi) {  // what lies behind the last token may be no number, and meets weights of zero
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (base + (x & 1 ? row_c : row_b) + 8 * (x >> 1) >= seg_hi)
+#pragma unroll
+            for (int w = 0; w < kVWords; ++w) vw[x][w] = 0;
+      }
+      refill();
       // channels 2x and 2x + 1 of this lane's chunk are output rows g and g + 8
 #pragma unroll
       for (int w = 0; w < kVWords; ++w) {
@@ -510,17 +533,18 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
     __syncthreads();
 
     // CTAs that share the item: the one it begins in and those that follow
-    const int64_t item_begin = seg.at - seg.tile0, item_end = item_begin + seg.tiles;
-    const int owner = static_cast<int>(ceil_div64((item_begin + 1) * parts, total) - 1);
+    const int64_t item_begin = seg.at - seg.unit0, item_end = item_begin + kItemTiles + seg.tiles;
+    const int owner = static_cast<int>(quotient((item_begin + 1) * parts + total - 1, total) - 1);
     const int sharers =
-        seg.take == seg.tiles ? 1 : static_cast<int>(ceil_div64(item_end * parts, total) - 1) - owner + 1;
+        seg.units == kItemTiles + seg.tiles
+            ? 1
+            : static_cast<int>(quotient(item_end * parts + total - 1, total) - 1) - owner + 1;
     constexpr int kSlot = kRows * (DIM + 3);
     float* slot = p.partial + (static_cast<int64_t>(cta) * 2 + (item_begin >= begin ? 1 : 0)) * kSlot;
-    const auto store = [&](int64_t r, int d, float4 v, float top, float top_u, float sum) {
+    const auto store = [&](int r, int d, float4 v, float top, float top_u, float sum) {
       if (r >= rows) return;
       const float inv = sum == 0.0f ? 0.0f : exp2_approx(top - top_u) / sum;
-      const int64_t row = (seg.s.first + r / p.group) * static_cast<int64_t>(p.kv_heads * p.group) +
-                          seg.head * p.group + r % p.group;
+      const int64_t row = output_row(p, seg.s, seg.head, r);
       uint2 w;
       if (p.q_bf16) {
         const __nv_bfloat162 a = __floats2bfloat162_rn(v.x * inv, v.y * inv);
@@ -683,7 +707,8 @@ bool shapes_ok(int64_t tokens, int64_t batch, int64_t max_new, int64_t q_heads, 
   if (tokens < 0 || tokens > INT32_MAX / 2 || batch < 0 || batch > (1 << 20) || max_new < 0) return false;
   if (kv_heads < 1 || kv_heads > 65536 || q_heads < kv_heads || q_heads > 65536 || q_heads % kv_heads) return false;
   if ((dim != 64 && dim != 128) || (page != 16 && page != 32 && page != 64 && page != 128)) return false;
-  return width >= 0 && width * page <= INT32_MAX / 2;
+  // rows of q and tokens of a table are counted in 32 bits
+  return tokens * q_heads <= INT32_MAX / 2 && width >= 0 && width <= INT32_MAX / 2 / page;
 }
 
 }  // namespace

@@ -63,6 +63,12 @@ __device__ __forceinline__ void row_bounds(const AttendParams& p, const Sequence
   lo = p.window > 0 ? static_cast<int>(min(max(position - p.window + 1, int64_t(0)), static_cast<int64_t>(s.hi))) : 0;
 }
 
+// Row r of (sequence, kv head) in the output and in lse.
+__device__ __forceinline__ int output_row(const AttendParams& p, const Sequence& s, int head, int r) {
+  const int token = r / p.group;
+  return (s.first + token) * (p.kv_heads * p.group) + head * p.group + (r - token * p.group);
+}
+
 // A row's power of two: q * factor is below 2 in magnitude (4 at the very top
 // of the range), and q = (q * factor) * gain.
 __device__ __forceinline__ void row_power(uint32_t top_bits, float& factor, float& gain) {

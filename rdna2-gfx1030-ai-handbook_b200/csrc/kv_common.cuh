@@ -18,6 +18,13 @@ constexpr float kScaleFloor = 7.888609052210118e-31f;  // 2^-100
 constexpr int kWarp = 32;
 constexpr unsigned kFullMask = 0xffffffffu;
 
+// a / b of non-negative numbers, in 32 bits where they fit: a 64-bit division
+// is a hundred instructions.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
 inline __host__ __device__ int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ------------------------------------------------------------ 16-byte vectors

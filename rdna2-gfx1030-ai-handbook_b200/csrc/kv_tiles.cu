@@ -65,7 +65,7 @@ struct TilesShared {
 struct Block {
   Sequence s;
   int b;
-  int64_t row0, rows;   // its first row, and the rows of the sequence
+  int row0, rows;       // its first row, and the rows of the sequence
   int tile0, tiles;
 };
 
@@ -74,8 +74,7 @@ struct Block {
 // stream through the first-level cache.
 struct Work {
   Block blk;
-  int64_t slot;
-  int head, split, parts;
+  int slot, head, split, parts;
 };
 
 struct TilesControl {
@@ -95,25 +94,31 @@ constexpr int kTilesBytes = TilesShared<DIM>::kOffCtl + static_cast<int>(sizeof(
 
 struct TilesParams {
   AttendParams a;
-  int64_t slots;  // row blocks of all sequences, at most
+  int slots;      // row blocks of all sequences, at most
   int splits;     // parts of the cached tokens that a row block is split into
   float* partial; // [slots][heads][splits][256][DIM] sums, then [..][3][256] m, n, l
   int* status;
 };
 
-// Slot s of the call is a row block of the sequence with first_block(b) <= s.
-__device__ __forceinline__ int64_t first_block(const AttendParams& p, int b) {
-  return static_cast<int64_t>(p.tok.begin(b)) * p.group / kCtaRows + b;
+// m, n and l of the parts, behind their sums.
+template <int DIM>
+__device__ __forceinline__ float* part_stats(const TilesParams& p) {
+  return p.partial + static_cast<int64_t>(p.slots) * p.a.kv_heads * p.splits * kCtaRows * DIM;
 }
 
-__device__ __forceinline__ bool load_block(const AttendParams& p, int64_t slot, Block& k) {
+// Slot s of the call is a row block of the sequence with first_block(b) <= s.
+__device__ __forceinline__ int first_block(const AttendParams& p, int b) {
+  return p.tok.begin(b) * p.group / kCtaRows + b;
+}
+
+__device__ __forceinline__ bool load_block(const AttendParams& p, int slot, Block& k) {
   k.b = warp_search(p.tok.batch, slot, [&](int i) { return first_block(p, i); });
   k.s = load_sequence(p, k.b);
-  k.rows = static_cast<int64_t>(k.s.count) * p.group;
+  k.rows = k.s.count * p.group;
   k.row0 = (slot - first_block(p, k.b)) * kCtaRows;
   if (k.row0 >= k.rows) return false;
   int lo, hi, unused;
-  const int64_t last = min(k.row0 + kCtaRows, k.rows) - 1;
+  const int last = min(k.row0 + kCtaRows, k.rows) - 1;
   row_bounds(p, k.s, k.s.start + k.row0 / p.group, lo, unused);
   row_bounds(p, k.s, k.s.start + last / p.group, unused, hi);
   k.tile0 = lo / kTileTokens;
@@ -126,10 +131,6 @@ __device__ __forceinline__ int part_tiles(const TilesParams& p, int tiles) { ret
 __device__ __forceinline__ int part_count(const TilesParams& p, int tiles) {
   const int per = part_tiles(p, tiles);
   return per ? (tiles + per - 1) / per : 1;
-}
-
-__device__ __forceinline__ int64_t output_row(const AttendParams& p, const Sequence& s, int head, int64_t r) {
-  return (s.first + r / p.group) * static_cast<int64_t>(p.kv_heads * p.group) + head * p.group + r % p.group;
 }
 
 __device__ __forceinline__ uint32_t swizzled(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
@@ -190,11 +191,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
   // the heaviest blocks of a causal prompt, its last rows, come first
   int count, token0;
   {
-    const int64_t unit = blockIdx.x;
+    const int unit = blockIdx.x, item = unit / tp.splits, from_last = item / p.kv_heads;
     Work mine;
-    mine.split = static_cast<int>(unit % tp.splits);
-    mine.head = static_cast<int>(unit / tp.splits % p.kv_heads);
-    mine.slot = tp.slots - 1 - unit / tp.splits / p.kv_heads;
+    mine.split = unit - item * tp.splits;
+    mine.head = item - from_last * p.kv_heads;
+    mine.slot = tp.slots - 1 - from_last;
     if (!load_block(p, mine.slot, mine.blk)) return;
     mine.parts = part_count(tp, mine.blk.tiles);
     if (mine.split >= mine.parts) return;
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
   constexpr int kChunks = DIM / 16;  // 16-byte pieces of half a row
   uint4 qv[kChunks];
   if (warp < kSoftmaxWarps) {
-    const int64_t r = blk.row0 + cta_row;
+    const int r = blk.row0 + cta_row;
     const bool valid = r < blk.rows;
     uint32_t top = 0;
     const uint16_t* src = static_cast<const uint16_t*>(p.q) + (blk.s.first + r / p.group) * p.q_token +
@@ -609,16 +610,15 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
       tc_fence_after();
       l += ctl.row[0][other][cta_row];
       const float inv = l == 0.0f ? 0.0f : exp2_approx(m - n) / l;
-      const int64_t r = blk.row0 + cta_row;
+      const int r = blk.row0 + cta_row;
       const bool valid = r < blk.rows;
       const int64_t out_row = output_row(p, blk.s, work.head, r);
       float* sums = nullptr;
       if (work.parts > 1) {
-        const int64_t part = (work.slot * p.kv_heads + work.head) * tp.splits + work.split;
+        const int64_t part = static_cast<int64_t>(work.slot * p.kv_heads + work.head) * tp.splits + work.split;
         sums = tp.partial + (part * kCtaRows + cta_row) * DIM + half * (DIM / 2);
         if (half == 0) {
-          float* stats =
-              tp.partial + tp.slots * p.kv_heads * tp.splits * kCtaRows * DIM + part * 3 * kCtaRows + cta_row;
+          float* stats = part_stats<DIM>(tp) + part * 3 * kCtaRows + cta_row;
           stats[0] = m;
           stats[kCtaRows] = n;
           stats[2 * kCtaRows] = l;
@@ -664,18 +664,17 @@ template <int DIM>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(TilesParams tp) {
   constexpr int kRowsEach = kJoinThreads / (DIM / 4);
   const AttendParams& p = tp.a;
-  const int64_t item = blockIdx.x / (kCtaRows / kRowsEach);
-  const int head = static_cast<int>(item % p.kv_heads);
-  const int64_t slot = item / p.kv_heads;
+  const int item = blockIdx.x / (kCtaRows / kRowsEach), slot = item / p.kv_heads;
+  const int head = item - slot * p.kv_heads;
   Block blk;
   if (!load_block(p, slot, blk)) return;
   const int parts = part_count(tp, blk.tiles);
   const int rr = blockIdx.x % (kCtaRows / kRowsEach) * kRowsEach + threadIdx.x / (DIM / 4);
-  const int64_t r = blk.row0 + rr;
+  const int r = blk.row0 + rr;
   if (parts == 1 || r >= blk.rows) return;
   const int d = threadIdx.x % (DIM / 4) * 4;
-  const int64_t part0 = item * tp.splits;
-  const float* stats = tp.partial + tp.slots * p.kv_heads * tp.splits * kCtaRows * DIM + part0 * 3 * kCtaRows + rr;
+  const int64_t part0 = static_cast<int64_t>(item) * tp.splits;
+  const float* stats = part_stats<DIM>(tp) + part0 * 3 * kCtaRows + rr;
   float m = -INFINITY, n = -INFINITY, l = 0.0f;
   for (int i = 0; i < parts; ++i) {
     m = fmaxf(m, stats[i * 3 * kCtaRows]);
@@ -718,8 +717,8 @@ template <int DIM, int CODE, int SEG>
 cudaError_t launch_tiles(const TilesParams& tp, cudaStream_t stream) {
   constexpr int kBytes = kTilesBytes<DIM>;
   static_assert(kBytes <= 227 * 1024, "a tile's operands do not fit in shared memory");
-  const int64_t items = tp.slots * tp.a.kv_heads;
-  if (items * tp.splits > INT32_MAX) return cudaErrorInvalidValue;
+  const int64_t items = static_cast<int64_t>(tp.slots) * tp.a.kv_heads;
+  if (items * tp.splits > INT32_MAX / 32) return cudaErrorInvalidValue;
   static const cudaError_t ready =
       cudaFuncSetAttribute(kv_tiles_kernel<DIM, CODE, SEG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
   if (ready != cudaSuccess) return ready;
@@ -749,7 +748,7 @@ size_t tiles_workspace_bytes(int64_t tokens, int64_t batch, int64_t group, int64
 cudaError_t run_tiles(const AttendParams& p, int dim, int code, void* workspace, cudaStream_t stream) {
   TilesParams tp{};
   tp.a = p;
-  tp.slots = block_slots(p.tok.tokens, p.tok.batch, p.group);
+  tp.slots = static_cast<int>(block_slots(p.tok.tokens, p.tok.batch, p.group));
   tp.splits = tile_splits(p.tok.tokens, p.tok.batch, p.group, p.kv_heads, p.width, 1 << p.page_shift);
   tp.partial = static_cast<float*>(workspace);
   tp.status = status_word_ptr();

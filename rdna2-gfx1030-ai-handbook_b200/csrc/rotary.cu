@@ -39,9 +39,9 @@ constexpr int kRotaryThreads = 128;
 template <typename T>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_vec_kernel(RotaryParams p, int lanes_row, int chunks) {
   constexpr int V = Vec<T>::kN;
-  const int64_t warp = (static_cast<int64_t>(blockIdx.x) * kRotaryThreads + threadIdx.x) / kWarp;
+  const uint32_t warp = blockIdx.x * (kRotaryThreads / kWarp) + threadIdx.x / kWarp;
   const int lane = threadIdx.x % kWarp;
-  const int64_t token = warp / chunks;
+  const int64_t token = warp / static_cast<uint32_t>(chunks);
   if (token >= p.tokens) return;
   const int rows = kWarp / lanes_row;  // heads at once
   const int u = lane % lanes_row;
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_vec_kernel(RotaryParams
 #pragma unroll
     for (int i = 0; i < V; ++i) sin[i] *= p.sign;
   }
-  const int head0 = static_cast<int>(warp % chunks) * rows * kRotaryUnroll + lane / lanes_row;
+  const int head0 = static_cast<int>(warp - token * chunks) * rows * kRotaryUnroll + lane / lanes_row;
   const T* x = static_cast<const T*>(p.x) + token * p.x_token;
   T* out = static_cast<T*>(p.out) + token * p.out_token;
   uint4 va[kRotaryUnroll], vb[kRotaryUnroll];
@@ -133,7 +133,7 @@ cudaError_t run_rotary(const RotaryParams& p, cudaStream_t stream) {
     threads = p.tokens * p.heads * (p.dim - p.rot / 2);
   }
   const int64_t blocks = ceil_div64(threads, kRotaryThreads);
-  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
+  if (blocks > INT32_MAX / (kRotaryThreads / kWarp)) return cudaErrorInvalidValue;  // warps are counted in 32 bits
   const dim3 grid(static_cast<unsigned>(blocks));
   if (vec) {
     rotary_vec_kernel<T><<<grid, kRotaryThreads, 0, stream>>>(p, lanes_row, chunks);
