@@ -74,7 +74,7 @@ int b2_kv_read(const void* k_codes, const void* v_codes, const float* k_scale, c
  * before its first call; every call leaves it ready for the next one on the
  * same stream, of any shape that it is large enough for. */
 size_t b2_kv_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t max_new, int64_t q_heads,
-                                       int64_t kv_heads, int64_t dim, int64_t width, int64_t page);
+                                       int64_t kv_heads, int64_t dim, int64_t width, int64_t page, int64_t window);
 int b2_kv_attention(const void* q, int dtype, int64_t tokens, int64_t q_heads, int64_t q_token_stride,
                     int64_t q_head_stride, const int32_t* lengths, const int32_t* offsets, int64_t batch,
                     int64_t max_new, const int32_t* table, int64_t width, int code, const void* k_codes,

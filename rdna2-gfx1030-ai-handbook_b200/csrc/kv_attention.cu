@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
   };
   const auto issue = [&](int i, int block) {
     const int stage = issued % kRing;
-    if (lane == 0) {
+    if (elect_one()) {
       sh.block[warp][stage] = block;
       uint64_t* bar = &sh.full[warp][stage];
       if (block >= 0) {
@@ -667,9 +667,11 @@ cudaError_t run_rows_any(const AttendParams& p, int dim, int code, int nt, int g
   return code == kCodeInt8 ? run_rows_nt<128, kCodeInt8>(p, nt, grid, s) : run_rows_nt<128, kCodeE4M3>(p, nt, grid, s);
 }
 
-// Most query rows of a (sequence, kv head) that kv_rows_kernel takes; it
-// reads the cache once for every 16 of them.
-constexpr int64_t kRowsMost = 32;
+// Most query rows of a (sequence, kv head) that kv_rows_kernel takes: what
+// one of its passes over the cache serves.  Measured for 24 rows, the two
+// kernels are level (8 heads over 32768 tokens 74 and 73 us, 16 sequences of
+// 4096 tokens 113 and 103 us), and from 32 rows on the tiles are ahead.
+constexpr int64_t kRowsMost = 16;
 
 // How a call is launched: on tensor-core tiles, or with `nt` times 8 columns
 // on `grid` CTAs.
@@ -680,14 +682,14 @@ struct Plan {
 };
 
 Plan make_plan(int64_t tokens, int64_t batch, int64_t max_new, int64_t q_heads, int64_t kv_heads, int64_t dim,
-               int64_t width, int64_t page) {
+               int64_t width, int64_t page, int64_t window) {
   Plan plan{};
   const int64_t group = q_heads / kv_heads;
   plan.tiles = max_new * group > kRowsMost;
   if (plan.tiles) {
     plan.workspace = kRowsMaxGrid * sizeof(int) + tiles_workspace_bytes(tokens, batch, group, kv_heads,
                                                                         static_cast<int>(dim), width,
-                                                                        static_cast<int>(page));
+                                                                        static_cast<int>(page), window);
     return plan;
   }
   plan.nt = max_new * group <= 8 ? 1 : 2;
@@ -717,9 +719,11 @@ bool shapes_ok(int64_t tokens, int64_t batch, int64_t max_new, int64_t q_heads, 
 extern "C" {
 
 size_t b2_kv_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t max_new, int64_t q_heads,
-                                       int64_t kv_heads, int64_t dim, int64_t width, int64_t page) {
-  if (!b2::shapes_ok(tokens, batch, max_new, q_heads, kv_heads, dim, width, page) || tokens == 0) return 0;
-  return b2::make_plan(tokens, batch, max_new, q_heads, kv_heads, dim, width, page).workspace;
+                                       int64_t kv_heads, int64_t dim, int64_t width, int64_t page, int64_t window) {
+  if (!b2::shapes_ok(tokens, batch, max_new, q_heads, kv_heads, dim, width, page) || window < 0 || tokens == 0 ||
+      batch == 0)
+    return 0;
+  return b2::make_plan(tokens, batch, max_new, q_heads, kv_heads, dim, width, page, window).workspace;
 }
 
 int b2_kv_attention(const void* q, int dtype, int64_t tokens, int64_t q_heads, int64_t q_token_stride,
@@ -738,7 +742,7 @@ int b2_kv_attention(const void* q, int dtype, int64_t tokens, int64_t q_heads, i
   if (!q || !lengths || (!table && width) || !k_codes || !v_codes || !k_scale || !v_scale || !out) return invalid;
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(k_codes, 16) || !aligned(v_codes, 16)) return invalid;
   if (q_token_stride < 0 || q_head_stride < 0 || q_token_stride % 8 || q_head_stride % 8) return invalid;
-  const b2::Plan plan = b2::make_plan(tokens, batch, max_new, q_heads, kv_heads, dim, width, page);
+  const b2::Plan plan = b2::make_plan(tokens, batch, max_new, q_heads, kv_heads, dim, width, page, window);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < plan.workspace) return invalid;
   b2::AttendParams p{};
   p.tok = {lengths, offsets, static_cast<int>(batch), static_cast<int>(tokens), static_cast<int>(tokens / batch)};

@@ -152,7 +152,7 @@ __device__ __forceinline__ float weight_of(float m, float top) {
 // Tiles of 128 cached tokens x 256 query rows on the 5th-generation tensor
 // cores (kv_tiles.cu): the workspace and the launch of a call with many rows.
 size_t tiles_workspace_bytes(int64_t tokens, int64_t batch, int64_t group, int64_t kv_heads, int dim, int64_t width,
-                             int page);
+                             int page, int64_t window);
 cudaError_t run_tiles(const AttendParams& p, int dim, int code, void* workspace, cudaStream_t stream);
 
 }  // namespace b2

@@ -17,6 +17,8 @@
 //   warp 26         the scales of the next tiles' blocks
 //   warp 27         nothing: registers are shared out by groups of four warps
 //
+// A block of 128 rows or fewer uses row tile 0 alone.
+//
 // The two row tiles alternate on the tensor cores: while one is in its
 // softmax the other multiplies, and they take turns so that it stays that way
 // (left alone they fall into step, exponentials and products in turn for
@@ -85,6 +87,9 @@ struct TilesControl {
   uint32_t present[4];  // bit g: group g lies on a page of the cache
   Work work;
   float row[2][2][kCtaRows];  // what the two threads of a row tell each other
+  // a softmax thread's own: what it needs once a tile
+  int lo[kSoftmaxWarps * kWarp], hi[kSoftmaxWarps * kWarp];
+  float n[kSoftmaxWarps * kWarp], l[kSoftmaxWarps * kWarp], bias[kSoftmaxWarps * kWarp];
   uint32_t tmem;
   int abort, drained;
 };
@@ -207,14 +212,15 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
   __syncthreads();
   const Work& work = ctl.work;
   const Block& blk = work.blk;
+  const int used = blk.rows - blk.row0 > kTileRows ? 2 : 1;  // row tiles that hold rows
 
   if (warp == kMmaWarp) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&ctl.k_full[i], kConvertWarps);
         mbar_init(&ctl.v_full[i], kConvertWarps);
-        mbar_init(&ctl.k_free[i], 2);
-        mbar_init(&ctl.v_free[i], 2);
+        mbar_init(&ctl.k_free[i], used);
+        mbar_init(&ctl.v_free[i], used);
         mbar_init(&ctl.s_full[i], 1);
         mbar_init(&ctl.p_full[i], kSoftmaxWarps / 2);
         mbar_init(&ctl.o_done[i], 1);
@@ -328,12 +334,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
       }
       __syncwarp();
     };
-    bool ok = count == 0 || wait(&ctl.k_full[0], 0, kSiteMma);
-    if (ok && count > 0) {
+    const int todo = t < used ? count : 0;
+    bool ok = todo == 0 || wait(&ctl.k_full[0], 0, kSiteMma);
+    if (ok && todo > 0) {
       tc_fence_after();
       scores(0);
     }
-    for (int i = 0; ok && i < count; ++i) {
+    for (int i = 0; ok && i < todo; ++i) {
       ok = wait(&ctl.v_full[i & 1], (i >> 1) & 1, kSiteMma) && wait(&ctl.p_full[t], i & 1, kSiteMma);
       if (!ok) break;
       tc_fence_after();
@@ -464,7 +471,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
       done(&ctl.v_full[stage]);
       load(p.v_codes, at, vw);
     }
-  } else if (warp < kSoftmaxWarps) {
+  } else if (warp < 8 * used) {
     // ------------------------------------------------------- softmax
     more_registers<kSoftmaxRegs>();
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
@@ -473,34 +480,39 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
     const uint32_t o_col = tmem + lanes + 256 + tile * 128 + half * (DIM / 2);     // and channels
     const int pair = 1 + tile * 4 + warp % 4;  // named barrier of the two warps that share rows
     const int other = half ^ 1;
-    // what int8 keys without their sign add to a row's products
-    const float bias = CODE == kCodeInt8 ? -128.0f * (ctl.row[1][0][cta_row] + ctl.row[1][1][cta_row]) : 0.0f;
-    int lo = 0, hi = 0;
+    const int me = threadIdx.x;
     // references of t and u; a row that is not one of the sequence needs none
-    float m = 0.0f, n = 0.0f, l = 0.0f;
-    if (blk.row0 + cta_row < blk.rows) {
-      row_bounds(p, blk.s, blk.s.start + (blk.row0 + cta_row) / p.group, lo, hi);
-      m = n = -INFINITY;
+    float m = 0.0f;
+    {
+      int lo = 0, hi = 0;
+      if (blk.row0 + cta_row < blk.rows) {
+        row_bounds(p, blk.s, blk.s.start + (blk.row0 + cta_row) / p.group, lo, hi);
+        m = -INFINITY;
+      }
+      ctl.lo[me] = lo;
+      ctl.hi[me] = hi;
+      ctl.n[me] = m;
+      ctl.l[me] = 0.0f;
+      // what int8 keys without their sign add to a row's products
+      ctl.bias[me] = CODE == kCodeInt8 ? -128.0f * (ctl.row[1][0][cta_row] + ctl.row[1][1][cta_row]) : 0.0f;
     }
     bool ok = true;
     for (int i = 0; i < count; ++i) {
-      ok = wait(&ctl.info_full[i & 3], (i >> 2) & 1, kSiteEpilogue) &&
-           wait(&ctl.s_full[tile], i & 1, kSiteEpilogue) &&
-           (i + tile == 0 || wait(&ctl.turn[tile], (i + tile - 1) & 1, kSiteEpilogue));
-      ok = bar_and(pair, 2 * kWarp, ok);
-      if (!ok) break;
-      tc_fence_after();
+      // After a wait that gave up the loop goes on without waiting: the two
+      // warps of a row meet at the same barriers whatever either has seen.
+      ok = ok && wait(&ctl.info_full[i & 3], (i >> 2) & 1, kSiteEpilogue);
       const GroupInfo* info = ctl.info[i & 3] + half * (kHalfTokens / 16);
       const uint32_t present = ctl.present[i & 3] >> (half * (kHalfTokens / 16));
       const int base = token0 + i * kTileTokens + half * kHalfTokens;
       // every row of this warp sees every one of its tokens
-      const bool whole = __all_sync(kFullMask, lo <= base && base + kHalfTokens <= hi) && (present & 0xfu) == 0xfu;
+      const bool whole = __all_sync(kFullMask, ctl.lo[me] <= base && base + kHalfTokens <= ctl.hi[me]) &&
+                         (present & 0xfu) == 0xfu;
 
       // 32 scores; -inf where masked
       const auto fetch = [&](int c, uint32_t (&x)[32]) {
         tmem_read32(s_col + 32 * c, x);
         if (whole) return;
-        const uint32_t seen = bit_range(lo - base - 32 * c, hi - base - 32 * c) &
+        const uint32_t seen = bit_range(ctl.lo[me] - base - 32 * c, ctl.hi[me] - base - 32 * c) &
                               ((present >> (2 * c) & 1 ? 0xffffu : 0u) | (present >> (2 * c) & 2 ? 0xffff0000u : 0u));
 #pragma unroll
         for (int j = 0; j < 32; ++j) x[j] = seen >> j & 1 ? x[j] : kMinusInf;
@@ -509,12 +521,15 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
       // of zero would make NaN of a masked score.
       const auto factor = [&](const GroupInfo& g, float& a, float& d) {
         const float product = qs * g.ks;
-        d = bias * product;
+        d = ctl.bias[me] * product;
         a = product * key_gain<CODE>();
         a = a == 0.0f ? 1.17549435e-38f : a;
       };
+      ok = ok && wait(&ctl.s_full[tile], i & 1, kSiteEpilogue);
+      if (used == 2 && i + tile > 0) ok = ok && wait(&ctl.turn[tile], (i + tile - 1) & 1, kSiteEpilogue);
+      tc_fence_after();
       uint32_t w[kHalfTokens / 2];
-      float sum, ref, ref_n;
+      float sum, ref;
       bool raise = i == 0, last = true;  // last: the turn has not been passed on
       for (;;) {
         if (raise) {
@@ -539,11 +554,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
           ctl.row[1][half][cta_row] = top_u;
           named_bar_sync(pair, 2 * kWarp);
           const float next = fmaxf(m, fmaxf(top_t, ctl.row[0][other][cta_row]));
-          const float next_n = fmaxf(n, fmaxf(top_u, ctl.row[1][other][cta_row]));
+          const float next_n = fmaxf(ctl.n[me], fmaxf(top_u, ctl.row[1][other][cta_row]));
           const float alpha = weight_of(m, next);
-          l *= weight_of(n, next_n);
+          ctl.l[me] *= weight_of(ctl.n[me], next_n);
+          ctl.n[me] = next_n;
           m = next;
-          n = next_n;
           if (i > 0) {
 #pragma unroll 1
             for (int c = 0; c < DIM / 64; ++c) {
@@ -556,7 +571,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
           }
         }
         ref = m == -INFINITY ? 0.0f : m;
-        ref_n = n == -INFINITY ? 0.0f : n;
         float weights = 0.0f;
         sum = 0.0f;
         uint32_t sc[32];
@@ -597,18 +611,19 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
       }
       tc_fence_after();
       tmem_st32(p_col, w);
-      l = fmaf(sum, exp2_approx(ref - ctl.top_lv[i & 3] - ref_n), l);
+      const float n = ctl.n[me];
+      ctl.l[me] = fmaf(sum, exp2_approx(ref - ctl.top_lv[i & 3] - (n == -INFINITY ? 0.0f : n)), ctl.l[me]);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.p_full[tile]);
     }
     if (ok && count > 0) ok = wait(&ctl.o_done[tile], (count - 1) & 1, kSiteEpilogue);
-    ctl.row[0][half][cta_row] = l;
+    ctl.row[0][half][cta_row] = ctl.l[me];
     ok = bar_and(pair, 2 * kWarp, ok);
     if (ok) {
       tc_fence_after();
-      l += ctl.row[0][other][cta_row];
+      const float n = ctl.n[me], l = ctl.row[0][0][cta_row] + ctl.row[0][1][cta_row];
       const float inv = l == 0.0f ? 0.0f : exp2_approx(m - n) / l;
       const int r = blk.row0 + cta_row;
       const bool valid = r < blk.rows;
@@ -703,14 +718,25 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(TilesParams tp) {
 
 int64_t block_slots(int64_t tokens, int64_t batch, int64_t group) { return tokens * group / kCtaRows + batch; }
 
-// One part while the row blocks alone fill the device; else as many as fill
-// it, with four tiles a part at least at the longest that the table holds.
-int tile_splits(int64_t tokens, int64_t batch, int64_t group, int64_t kv_heads, int64_t width, int page) {
-  const int64_t items = block_slots(tokens, batch, group) * kv_heads;
-  const int64_t most = ceil_div64(ceil_div64(width * page, kTileTokens), 4);
-  const int64_t want = device_sm_count() / items;
-  const int64_t splits = want < most ? want : most;
-  return splits > 1 ? static_cast<int>(splits) : 1;
+// Parts that every row block's tokens are split into: the number that gives
+// the least time for CTAs of equal length, one an SM, where a part costs its
+// tiles and about kPartTiles more (its start, its end and its share of the
+// join).  Lengths are not known here: the longest that the table can hold, or
+// the window, stands for them.
+constexpr int64_t kPartTiles = 4, kMostParts = 64;
+
+int tile_splits(int64_t tokens, int64_t batch, int64_t group, int64_t kv_heads, int64_t width, int page,
+                int64_t window) {
+  const int64_t items = block_slots(tokens, batch, group) * kv_heads, sms = device_sm_count();
+  int64_t seen = width * page;
+  if (window > 0 && window + kCtaRows / group < seen) seen = window + kCtaRows / group;
+  const int64_t tiles = ceil_div64(seen, kTileTokens);
+  int64_t best = 1, least = ceil_div64(items, sms) * (tiles + kPartTiles);
+  for (int64_t s = 2; s <= kMostParts && s <= tiles && items * s <= 4 * sms; ++s) {
+    const int64_t time = ceil_div64(items * s, sms) * (ceil_div64(tiles, s) + kPartTiles) + kPartTiles;
+    if (time < least) best = s, least = time;
+  }
+  return static_cast<int>(best);
 }
 
 template <int DIM, int CODE, int SEG>
@@ -738,8 +764,8 @@ cudaError_t launch_tiles_page(const TilesParams& tp, cudaStream_t stream) {
 }  // namespace
 
 size_t tiles_workspace_bytes(int64_t tokens, int64_t batch, int64_t group, int64_t kv_heads, int dim, int64_t width,
-                             int page) {
-  const int splits = tile_splits(tokens, batch, group, kv_heads, width, page);
+                             int page, int64_t window) {
+  const int splits = tile_splits(tokens, batch, group, kv_heads, width, page, window);
   if (splits == 1) return 0;
   return static_cast<size_t>(block_slots(tokens, batch, group) * kv_heads * splits) * kCtaRows * (dim + 3) *
          sizeof(float);
@@ -749,7 +775,7 @@ cudaError_t run_tiles(const AttendParams& p, int dim, int code, void* workspace,
   TilesParams tp{};
   tp.a = p;
   tp.slots = static_cast<int>(block_slots(p.tok.tokens, p.tok.batch, p.group));
-  tp.splits = tile_splits(p.tok.tokens, p.tok.batch, p.group, p.kv_heads, p.width, 1 << p.page_shift);
+  tp.splits = tile_splits(p.tok.tokens, p.tok.batch, p.group, p.kv_heads, p.width, 1 << p.page_shift, p.window);
   tp.partial = static_cast<float*>(workspace);
   tp.status = status_word_ptr();
   const bool int8 = code == kCodeInt8;

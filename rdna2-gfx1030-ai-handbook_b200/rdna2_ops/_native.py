@@ -87,7 +87,7 @@ SIGNATURES = {
     "b2_kv_append": ([_p, _p, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _p, _i64, _p, _i64, _i64,
                       _i64, _p, _p, _i64, _i64, _int, _int, _p, _p, _p, _p, _i64, _i64, _p], _int),
     "b2_kv_read": ([_p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _p, _i64, _int, _p, _p, _p, _p], _int),
-    "b2_kv_attention_workspace_bytes": ([_i64] * 8, _size),
+    "b2_kv_attention_workspace_bytes": ([_i64] * 9, _size),
     "b2_kv_attention": ([_p, _int, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _int, _p, _p, _p, _p, _i64,
                          _i64, _i64, _i64, ctypes.c_float, _int, _i64, _p, _p, _p, _size, _p], _int),
     "b2_quant_linear_noalloc_max_bytes": ([], _size),

@@ -154,7 +154,7 @@ class PagedKVCache:
                 raise TypeError("q must have k's type and device")
             if q.ndim != 3 or q.shape[0] != tokens or q.shape[2] != self.head_dim:
                 raise ValueError(f"q must be [{tokens}, heads, {self.head_dim}], got {tuple(q.shape)}")
-            rotated = torch.empty(q.shape, device=dev, dtype=q.dtype)
+            rotated = torch.empty_like(q, memory_format=torch.contiguous_format)
             q = _rows(q) if q.numel() else None
         if tokens == 0:
             return rotated
@@ -199,12 +199,13 @@ class PagedKVCache:
             max_new = tokens
         elif max_new < 1:
             raise ValueError(f"max_new must be at least 1, got {max_new}")
-        out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = torch.empty((tokens, heads), device=dev, dtype=torch.float32) if return_lse else None
         if tokens:
             q = _rows(q)
             lib, stream = nat.library(), nat.stream_ptr(dev)
-            need = _workspace_bytes(tokens, batch, max_new, heads, self.kv_heads, self.head_dim, width, self.page_size)
+            need = _workspace_bytes(tokens, batch, max_new, heads, self.kv_heads, self.head_dim, width,
+                                    self.page_size, window or 0)
             work = self._workspaces.get(stream)
             if work is None or work.numel() < need:
                 work = self._workspaces[stream] = torch.zeros(need, device=dev, dtype=torch.uint8)

@@ -99,7 +99,7 @@ def rotary(x, angles, positions, *, layout="half", inverse=False, out=None):
     if positions.shape != (tokens,) or not positions.is_contiguous():
         raise ValueError(f"positions must be contiguous [{tokens}], got {tuple(positions.shape)}")
     if out is None:
-        out = torch.empty((tokens, heads, dim), device=dev, dtype=x.dtype)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != dev or out.stride(2) != 1:
         raise ValueError("out must have x's shape, type and device, and contiguous channels")
     if x.stride(2) != 1:
