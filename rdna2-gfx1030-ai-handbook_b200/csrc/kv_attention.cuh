@@ -11,7 +11,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 // A softmax goes on with the reference it has while its weights (in the tile
 // kernel their sum over a tile) stay below this.
-constexpr float kMostWeight = 8192.0f;
+constexpr float kMostWeight = 49152.0f;
 
 struct AttendParams {
   Tokens tok;

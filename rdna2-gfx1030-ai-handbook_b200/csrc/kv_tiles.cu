@@ -44,6 +44,12 @@ constexpr int kTilesThreads = 28 * kWarp;
 // Registers a thread: 72 at launch, 4 * 80 + 2 * 64 + 56 = 7 * 72 afterwards.
 constexpr int kSoftmaxRegs = 80, kConvertRegs = 64, kOtherRegs = 56;
 constexpr int kHalfTokens = kTileTokens / 2;  // of a softmax thread
+// A reference is set this far above the tile's maximum.  Together with
+// kMostWeight it leaves 2^20 for what later tiles bring: going through a tile
+// twice costs as much as a tile, and with 2^13 a prompt whose keys are
+// unequally loud did so in every fourth of its first tiles.  Weights below
+// 2^-9 of the largest are subnormal fp16 then, off by 2^-20 of it at most.
+constexpr float kHeadroomLog2 = 5.0f;
 constexpr uint32_t kMinusInf = 0xff800000u;
 
 // One row tile of queries, or one tile of K or V: panels of 64 channels, 128
@@ -53,6 +59,13 @@ constexpr int kPanel = 128 * 128;
 struct __align__(16) GroupInfo {
   float ks, lv, iv, unused;  // key scale, log2 of the value scale, 2^(top_lv - lv)
 };
+
+// Tensor memory, 512 columns: scores of the row tiles at 0 and 128, sums at
+// 256, DIM columns each.  Heads of 64 leave 128 columns, so that the weights
+// have a place of their own and the next scores are on their way while they
+// are multiplied; with heads of 128 the weights overlay the scores.
+template <int DIM>
+constexpr bool kApart = DIM == 64;
 
 template <int DIM>
 struct TilesShared {
@@ -80,13 +93,14 @@ struct Work {
 };
 
 struct TilesControl {
-  uint64_t k_full[2], k_free[2], v_full[2], v_free[2];
-  uint64_t s_full[2], p_full[2], o_done[2], info_full[4], turn[2], last[2];
+  uint64_t q_full[2], k_full[2], k_free[2], v_full[2], v_free[2];
+  uint64_t s_full[2], s_read[2], p_full[2], o_done[2], info_full[4], turn[2], last[2];
   GroupInfo info[4][kGroups];
   float top_lv[4];
   uint32_t present[4];  // bit g: group g lies on a page of the cache
   Work work;
-  float row[2][2][kCtaRows];  // what the two threads of a row tell each other
+  // what the two threads of a row tell each other: maxima, and the sum of q
+  float row[2][2][kCtaRows], sum[2][kCtaRows];
   // a softmax thread's own: what it needs once a tile
   int lo[kSoftmaxWarps * kWarp], hi[kSoftmaxWarps * kWarp];
   float n[kSoftmaxWarps * kWarp], l[kSoftmaxWarps * kWarp], bias[kSoftmaxWarps * kWarp];
@@ -193,35 +207,29 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
   const uint32_t base_u32 = smem_u32(smem);
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
 
-  // the heaviest blocks of a causal prompt, its last rows, come first
-  int count, token0;
-  {
-    const int unit = blockIdx.x, item = unit / tp.splits, from_last = item / p.kv_heads;
-    Work mine;
-    mine.split = unit - item * tp.splits;
-    mine.head = item - from_last * p.kv_heads;
-    mine.slot = tp.slots - 1 - from_last;
-    if (!load_block(p, mine.slot, mine.blk)) return;
-    mine.parts = part_count(tp, mine.blk.tiles);
-    if (mine.split >= mine.parts) return;
-    const int per = part_tiles(tp, mine.blk.tiles), first = mine.split * per;
-    count = min(per, mine.blk.tiles - first);
-    token0 = (mine.blk.tile0 + first) * kTileTokens;
-    if (threadIdx.x == 0) ctl.work = mine;
-  }
-  __syncthreads();
-  const Work& work = ctl.work;
-  const Block& blk = work.blk;
-  const int used = blk.rows - blk.row0 > kTileRows ? 2 : 1;  // row tiles that hold rows
-
+  const int unit = blockIdx.x, item = unit / tp.splits, from_last = item / p.kv_heads;
+  Work mine;
+  mine.split = unit - item * tp.splits;
+  mine.head = item - from_last * p.kv_heads;
+  mine.slot = tp.slots - 1 - from_last;  // the heaviest blocks of a causal prompt, its last rows, come first
+  if (!load_block(p, mine.slot, mine.blk)) return;
+  mine.parts = part_count(tp, mine.blk.tiles);
+  if (mine.split >= mine.parts) return;
+  const int per = part_tiles(tp, mine.blk.tiles), first = mine.split * per;
+  const int count = min(per, mine.blk.tiles - first);
+  const int token0 = (mine.blk.tile0 + first) * kTileTokens;
+  const int used = mine.blk.rows - mine.blk.row0 > kTileRows ? 2 : 1;  // row tiles that hold rows
+  if (threadIdx.x == 0) ctl.work = mine;
   if (warp == kMmaWarp) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
+        mbar_init(&ctl.q_full[i], kSoftmaxWarps / 2);
         mbar_init(&ctl.k_full[i], kConvertWarps);
         mbar_init(&ctl.v_full[i], kConvertWarps);
         mbar_init(&ctl.k_free[i], used);
         mbar_init(&ctl.v_free[i], used);
         mbar_init(&ctl.s_full[i], 1);
+        mbar_init(&ctl.s_read[i], kSoftmaxWarps / 2);
         mbar_init(&ctl.p_full[i], kSoftmaxWarps / 2);
         mbar_init(&ctl.o_done[i], 1);
         mbar_init(&ctl.turn[i], kSoftmaxWarps / 2);
@@ -235,61 +243,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
     tmem_alloc(&ctl.tmem, 512);
     tmem_relinquish();
   }
-
-  // ---- queries: a softmax thread brings half of its row's channels
-  const int tile = warp / 8, half = warp / 4 % 2, row = threadIdx.x % kTileRows;
-  const int cta_row = tile * kTileRows + row;
-  constexpr int kChunks = DIM / 16;  // 16-byte pieces of half a row
-  uint4 qv[kChunks];
-  if (warp < kSoftmaxWarps) {
-    const int r = blk.row0 + cta_row;
-    const bool valid = r < blk.rows;
-    uint32_t top = 0;
-    const uint16_t* src = static_cast<const uint16_t*>(p.q) + (blk.s.first + r / p.group) * p.q_token +
-                          (work.head * p.group + r % p.group) * p.q_head + half * (DIM / 2);
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      qv[c] = valid ? ldg_v4(src + 8 * c) : make_uint4(0, 0, 0, 0);
-      float f[8];
-      if (p.q_bf16) {
-        Vec<__nv_bfloat16>::unpack(qv[c], f);
-      } else {
-        Vec<__half>::unpack(qv[c], f);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-    }
-    ctl.row[0][half][cta_row] = __uint_as_float(top);
-  }
-  __syncthreads();
-  float qs = 0.0f;
-  if (warp < kSoftmaxWarps) {
-    float factor, gain, sum = 0.0f;
-    row_power(max(__float_as_uint(ctl.row[0][0][cta_row]), __float_as_uint(ctl.row[0][1][cta_row])), factor, gain);
-    qs = gain * p.scale_log2;
-    uint8_t* dst = smem + Shared::kOffQ + tile * Shared::kTile;
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      float f[8];
-      if (p.q_bf16) {
-        Vec<__nv_bfloat16>::unpack(qv[c], f);
-      } else {
-        Vec<__half>::unpack(qv[c], f);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        f[i] *= factor;
-        sum += __half2float(__float2half_rn(f[i]));
-      }
-      const int chunk = half * kChunks + c;
-      *reinterpret_cast<uint4*>(dst + chunk / 8 * kPanel + swizzled(row, chunk % 8)) = Vec<__half>::pack(f);
-    }
-    ctl.row[1][half][cta_row] = sum;
-    fence_proxy_async_smem();
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  const Work& work = ctl.work;
+  const Block& blk = work.blk;
   const uint32_t tmem = ctl.tmem;
   volatile int* abort_flag = &ctl.abort;
   // called by a whole warp, which leaves with one answer
@@ -309,6 +267,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
     constexpr uint32_t kIdescS = make_idesc<kKindF16>(kTileRows, kTileTokens);
     constexpr uint32_t kIdescO = make_idesc<kKindF16>(kTileRows, DIM) | (1u << 16);  // V: N contiguous
     const int t = warp - kMmaWarp;
+    const uint32_t weights = tmem + (kApart<DIM> ? 384 + t * 64 : t * 128);
     const auto scores = [&](int stage) {
       if (elect_one()) {
         const uint32_t q = base_u32 + Shared::kOffQ + t * Shared::kTile;
@@ -328,30 +287,32 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
         const uint32_t v = base_u32 + Shared::kOffV + stage * Shared::kTile;
 #pragma unroll
         for (int x = 0; x < kTileTokens / 16; ++x)
-          umma_ts_f16(tmem + 256 + t * 128, tmem + t * 128 + 8 * x, channels_desc(v + x * 2048), kIdescO, add || x > 0);
+          umma_ts_f16(tmem + 256 + t * DIM, weights + 8 * x, channels_desc(v + x * 2048), kIdescO, add || x > 0);
         umma_commit(&ctl.o_done[t]);
         umma_commit(&ctl.v_free[stage]);
       }
       __syncwarp();
     };
     const int todo = t < used ? count : 0;
-    bool ok = todo == 0 || wait(&ctl.k_full[0], 0, kSiteMma);
+    bool ok = todo == 0 || (wait(&ctl.q_full[t], 0, kSiteMma) && wait(&ctl.k_full[0], 0, kSiteMma));
     if (ok && todo > 0) {
       tc_fence_after();
       scores(0);
     }
     for (int i = 0; ok && i < todo; ++i) {
-      ok = wait(&ctl.v_full[i & 1], (i >> 1) & 1, kSiteMma) && wait(&ctl.p_full[t], i & 1, kSiteMma);
+      const auto next_scores = [&](uint64_t* before) {
+        ok = wait(&ctl.k_full[(i + 1) & 1], ((i + 1) >> 1) & 1, kSiteMma) && wait(before, i & 1, kSiteMma);
+        if (!ok) return;
+        tc_fence_after();
+        scores((i + 1) & 1);
+      };
+      if (kApart<DIM> && i + 1 < todo) next_scores(&ctl.s_read[t]);
+      ok = ok && wait(&ctl.v_full[i & 1], (i >> 1) & 1, kSiteMma) && wait(&ctl.p_full[t], i & 1, kSiteMma);
       if (!ok) break;
       tc_fence_after();
       output(i & 1, i > 0);
-      if (i + 1 < count) {
-        // the weights lie where the next scores go: they have been read first
-        ok = wait(&ctl.k_full[(i + 1) & 1], ((i + 1) >> 1) & 1, kSiteMma) && wait(&ctl.o_done[t], i & 1, kSiteMma);
-        if (!ok) break;
-        tc_fence_after();
-        scores((i + 1) & 1);
-      }
+      // the weights lie where the next scores go: they have been read first
+      if (!kApart<DIM> && i + 1 < todo) next_scores(&ctl.o_done[t]);
     }
     // nothing is in flight when tensor memory is given back, after a wait
     // that gave up either
@@ -474,12 +435,65 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
   } else if (warp < 8 * used) {
     // ------------------------------------------------------- softmax
     more_registers<kSoftmaxRegs>();
+    const int tile = warp / 8, half = warp / 4 % 2, row = threadIdx.x % kTileRows;
+    const int cta_row = tile * kTileRows + row, other = half ^ 1;
+    const int pair = 1 + tile * 4 + warp % 4;  // named barrier of the two warps that share rows
+    // a thread brings half of its row's channels
+    float qs;
+    {
+      constexpr int kChunks = DIM / 16;  // 16-byte pieces of half a row
+      const int r = blk.row0 + cta_row;
+      const bool valid = r < blk.rows;
+      const uint16_t* src = static_cast<const uint16_t*>(p.q) +
+                            static_cast<int64_t>(blk.s.first + r / p.group) * p.q_token +
+                            (work.head * p.group + r % p.group) * p.q_head + half * (DIM / 2);
+      uint4 v[kChunks];
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) v[c] = valid ? ldg_v4(src + 8 * c) : make_uint4(0, 0, 0, 0);
+      const auto unpack = [&](int c, float (&f)[8]) {
+        if (p.q_bf16) {
+          Vec<__nv_bfloat16>::unpack(v[c], f);
+        } else {
+          Vec<__half>::unpack(v[c], f);
+        }
+      };
+      uint32_t top = 0;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        float f[8];
+        unpack(c, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+      }
+      ctl.row[0][half][cta_row] = __uint_as_float(top);
+      named_bar_sync(pair, 2 * kWarp);
+      float factor, gain, sum = 0.0f;
+      row_power(max(top, __float_as_uint(ctl.row[0][other][cta_row])), factor, gain);
+      qs = gain * p.scale_log2;
+      uint8_t* dst = smem + Shared::kOffQ + tile * Shared::kTile;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        float f[8];
+        unpack(c, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] *= factor;
+        const uint4 h = Vec<__half>::pack(f);
+        if (CODE == kCodeInt8) {
+          Vec<__half>::unpack(h, f);
+          sum += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+        }
+        const int chunk = half * kChunks + c;
+        *reinterpret_cast<uint4*>(dst + chunk / 8 * kPanel + swizzled(row, chunk % 8)) = h;
+      }
+      ctl.sum[half][cta_row] = sum;
+      fence_proxy_async_smem();
+      named_bar_sync(pair, 2 * kWarp);
+      if (lane == 0) mbar_arrive(&ctl.q_full[tile]);
+    }
     const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
     const uint32_t s_col = tmem + lanes + tile * 128 + half * kHalfTokens;         // this thread's scores,
-    const uint32_t p_col = tmem + lanes + tile * 128 + half * (kHalfTokens / 2);   // weights
-    const uint32_t o_col = tmem + lanes + 256 + tile * 128 + half * (DIM / 2);     // and channels
-    const int pair = 1 + tile * 4 + warp % 4;  // named barrier of the two warps that share rows
-    const int other = half ^ 1;
+    const uint32_t p_col = tmem + lanes + (kApart<DIM> ? 384 + tile * 64 : tile * 128) + half * (kHalfTokens / 2);
+    const uint32_t o_col = tmem + lanes + 256 + tile * DIM + half * (DIM / 2);     // weights and channels
     const int me = threadIdx.x;
     // references of t and u; a row that is not one of the sequence needs none
     float m = 0.0f;
@@ -494,7 +508,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
       ctl.n[me] = m;
       ctl.l[me] = 0.0f;
       // what int8 keys without their sign add to a row's products
-      ctl.bias[me] = CODE == kCodeInt8 ? -128.0f * (ctl.row[1][0][cta_row] + ctl.row[1][1][cta_row]) : 0.0f;
+      ctl.bias[me] = CODE == kCodeInt8 ? -128.0f * (ctl.sum[0][cta_row] + ctl.sum[1][cta_row]) : 0.0f;
     }
     bool ok = true;
     for (int i = 0; i < count; ++i) {
@@ -553,13 +567,17 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
           ctl.row[0][half][cta_row] = top_t;
           ctl.row[1][half][cta_row] = top_u;
           named_bar_sync(pair, 2 * kWarp);
-          const float next = fmaxf(m, fmaxf(top_t, ctl.row[0][other][cta_row]));
+          const float next = fmaxf(m, fmaxf(top_t, ctl.row[0][other][cta_row]) + kHeadroomLog2);
           const float next_n = fmaxf(ctl.n[me], fmaxf(top_u, ctl.row[1][other][cta_row]));
           const float alpha = weight_of(m, next);
           ctl.l[me] *= weight_of(ctl.n[me], next_n);
           ctl.n[me] = next_n;
           m = next;
           if (i > 0) {
+            if (kApart<DIM>) {
+              ok = ok && wait(&ctl.o_done[tile], (i - 1) & 1, kSiteEpilogue);
+              tc_fence_after();
+            }
 #pragma unroll 1
             for (int c = 0; c < DIM / 64; ++c) {
               uint32_t o[32];
@@ -608,6 +626,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
         if (bar_and(pair, 2 * kWarp, fits)) break;
         raise = true;
         last = false;
+      }
+      if (kApart<DIM>) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.s_read[tile]);
+        if (i > 0) ok = ok && wait(&ctl.o_done[tile], (i - 1) & 1, kSiteEpilogue);
       }
       tc_fence_after();
       tmem_st32(p_col, w);
