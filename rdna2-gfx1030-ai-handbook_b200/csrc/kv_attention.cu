@@ -644,9 +644,9 @@ bool encode_codes(CUtensorMap* map, const void* codes, int64_t blocks, int page)
 template <int DIM, int CODE, int NT>
 cudaError_t run_rows(const AttendParams& p, int grid, cudaStream_t stream) {
   constexpr int kBytes = sizeof(RowsShared<DIM, NT>) + 1024;
-  static const cudaError_t ready = cudaFuncSetAttribute(
-      kv_rows_kernel<DIM, CODE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-  if (ready != cudaSuccess) return ready;
+  static bool ready[64] = {};
+  const cudaError_t e = allow_shared(reinterpret_cast<const void*>(kv_rows_kernel<DIM, CODE, NT>), kBytes, ready);
+  if (e != cudaSuccess) return e;
   CUtensorMap k_map{}, v_map{};
   const int64_t blocks = p.pages * p.kv_heads;
   if (blocks > 0 && !(encode_codes<DIM>(&k_map, p.k_codes, blocks, 1 << p.page_shift) &&

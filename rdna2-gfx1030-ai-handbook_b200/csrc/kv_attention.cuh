@@ -149,6 +149,19 @@ __device__ __forceinline__ float weight_of(float m, float top) {
   return top == -INFINITY ? 0.0f : exp2_approx(m - top);
 }
 
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device,
+// once for each device (`done`, one entry a device).
+inline cudaError_t allow_shared(const void* kernel, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (done[dev]) return cudaSuccess;
+  const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  done[dev] = set == cudaSuccess;
+  return set;
+}
+
 // Tiles of 128 cached tokens x 256 query rows on the 5th-generation tensor
 // cores (kv_tiles.cu): the workspace and the launch of a call with many rows.
 size_t tiles_workspace_bytes(int64_t tokens, int64_t batch, int64_t group, int64_t kv_heads, int dim, int64_t width,

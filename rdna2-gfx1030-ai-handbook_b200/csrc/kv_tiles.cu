@@ -768,11 +768,11 @@ cudaError_t launch_tiles(const TilesParams& tp, cudaStream_t stream) {
   static_assert(kBytes <= 227 * 1024, "a tile's operands do not fit in shared memory");
   const int64_t items = static_cast<int64_t>(tp.slots) * tp.a.kv_heads;
   if (items * tp.splits > INT32_MAX / 32) return cudaErrorInvalidValue;
-  static const cudaError_t ready =
-      cudaFuncSetAttribute(kv_tiles_kernel<DIM, CODE, SEG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-  if (ready != cudaSuccess) return ready;
+  static bool ready[64] = {};
+  cudaError_t e = allow_shared(reinterpret_cast<const void*>(kv_tiles_kernel<DIM, CODE, SEG>), kBytes, ready);
+  if (e != cudaSuccess) return e;
   kv_tiles_kernel<DIM, CODE, SEG><<<static_cast<unsigned>(items * tp.splits), kTilesThreads, kBytes, stream>>>(tp);
-  cudaError_t e = cudaGetLastError();
+  e = cudaGetLastError();
   if (e != cudaSuccess || tp.splits == 1) return e;
   constexpr int kBlocks = kCtaRows / (kJoinThreads / (DIM / 4));
   kv_join_kernel<DIM><<<static_cast<unsigned>(items * kBlocks), kJoinThreads, 0, stream>>>(tp);

@@ -138,7 +138,8 @@ def require_device(*tensors):
 def stream_ptr(device):
     """The current stream's cudaStream_t (the raw handle: torch.cuda.current_stream
     builds a Stream object for it, 3 us a call)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def check(status, what):

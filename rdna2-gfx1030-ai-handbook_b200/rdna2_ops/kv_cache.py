@@ -234,6 +234,6 @@ class PagedKVCache:
         scales = torch.empty((2, *shape[:2]), device=dev, dtype=torch.float32) if return_scales else None
         nat.check(nat.library().b2_kv_read(
             *self._memory()[:4], _CODE_INDEX[self.k_codes.dtype], self.num_pages, self.kv_heads, self.page_size,
-            self.head_dim, pages.data_ptr(), shape[0], nat.DTYPE_CODE[dtype], k.data_ptr(), v.data_ptr(), nat.ptr(scales),
-            nat.stream_ptr(dev)), "b2_kv_read")
+            self.head_dim, pages.data_ptr(), shape[0], nat.DTYPE_CODE[dtype], k.data_ptr(), v.data_ptr(),
+            nat.ptr(scales), nat.stream_ptr(dev)), "b2_kv_read")
         return (k, v, *scales.unbind()) if return_scales else (k, v)
