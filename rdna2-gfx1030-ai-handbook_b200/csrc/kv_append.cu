@@ -94,7 +94,7 @@ __device__ __forceinline__ void append_block(const AppendParams& p, uint32_t ite
   from = from > start ? from : start;
   from = from > 0 ? from : 0;
   to = to < start + count ? to : start + count;
-  if (from >= to || block >= p.width) return;
+  if (nth < 0 || from >= to || block >= p.width) return;  // nth < 0: offsets that decrease
   const int64_t page_id = __ldg(p.table + static_cast<int64_t>(b) * p.width + block);
 
   // this thread's rows of the block's new ones, kRows apart
@@ -173,8 +173,9 @@ __device__ __forceinline__ void append_block(const AppendParams& p, uint32_t ite
     for (int i = tid; i < words; i += THREADS) {
       const uint32_t w = row[i];
       float f[4];
+      code_values<CODE>(w, f);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) f[j] = __fmul_rn(from_code<CODE>((w >> (8 * j)) & 0xffu), ratio);
+      for (int j = 0; j < 4; ++j) f[j] = __fmul_rn(f[j], ratio);
       row[i] = pack_codes<CODE>(f, now);
     }
   }
@@ -312,11 +313,13 @@ cudaError_t run_append_dim(const AppendParams& p, int dim, int code, cudaStream_
 
 // ------------------------------------------------------------------ read back
 // Values of whole pages: [n][kv_heads][page][dim], K and V.
+constexpr int kReadThreads = 128;
+
 template <typename T, int CODE>
-__global__ void __launch_bounds__(256) read_kernel(const uint8_t* k_codes, const uint8_t* v_codes, const float* k_scale,
-                                                   const float* v_scale, const int32_t* pages, int64_t n,
-                                                   int64_t num_pages, int kv_heads, int block_bytes, T* k_out, T* v_out,
-                                                   float* scales_out) {
+__global__ void __launch_bounds__(kReadThreads)
+    read_kernel(const uint8_t* k_codes, const uint8_t* v_codes, const float* k_scale, const float* v_scale,
+                const int32_t* pages, int64_t n, int64_t num_pages, int kv_heads, int block_bytes, T* k_out, T* v_out,
+                float* scales_out) {
   const uint32_t item = blockIdx.x;  // (page, head, K or V)
   const bool is_v = item & 1;
   const int64_t i = (item >> 1) / static_cast<uint32_t>(kv_heads);
@@ -327,14 +330,19 @@ __global__ void __launch_bounds__(256) read_kernel(const uint8_t* k_codes, const
   const float scale = held ? (is_v ? v_scale : k_scale)[page * kv_heads + head] : __int_as_float(0x7fffffff);
   if (scales_out != nullptr && threadIdx.x == 0) scales_out[((is_v ? n : 0) + i) * kv_heads + head] = scale;
   const uint8_t* codes = (is_v ? v_codes : k_codes) + (held ? (page * kv_heads + head) * block_bytes : 0);
-  for (int e = threadIdx.x * 8; e < block_bytes; e += 256 * 8) {
-    const uint2 w = held ? *reinterpret_cast<const uint2*>(codes + e) : make_uint2(0, 0);
-    float f[8];
+#pragma unroll 2
+  for (int e = threadIdx.x * 16; e < block_bytes; e += kReadThreads * 16) {
+    const uint4 w = held ? ldg_v4(codes + e) : make_uint4(0, 0, 0, 0);
+    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+    float f[16];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      f[j] = __fmul_rn(from_code<CODE>(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xffu), scale);
+    for (int i = 0; i < 4; ++i) {
+      code_values<CODE>(word[i], f + 4 * i);
 #pragma unroll
-    for (int j = 0; j < 8; j += Vec<T>::kN) {
+      for (int j = 0; j < 4; ++j) f[4 * i + j] = __fmul_rn(f[4 * i + j], scale);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; j += Vec<T>::kN) {
       float part[Vec<T>::kN];
 #pragma unroll
       for (int x = 0; x < Vec<T>::kN; ++x) part[x] = f[j + x];
@@ -350,12 +358,14 @@ cudaError_t run_read(const uint8_t* kc, const uint8_t* vc, const float* ks, cons
   const int64_t grid = n * kv_heads * 2;
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
   const unsigned g = static_cast<unsigned>(grid);
+  T* k = static_cast<T*>(k_out);
+  T* v = static_cast<T*>(v_out);
   if (code == kCodeInt8) {
-    read_kernel<T, kCodeInt8><<<g, 256, 0, stream>>>(kc, vc, ks, vs, pages, n, num_pages, kv_heads, block_bytes,
-                                                     static_cast<T*>(k_out), static_cast<T*>(v_out), scales);
+    read_kernel<T, kCodeInt8><<<g, kReadThreads, 0, stream>>>(kc, vc, ks, vs, pages, n, num_pages, kv_heads,
+                                                              block_bytes, k, v, scales);
   } else {
-    read_kernel<T, kCodeE4M3><<<g, 256, 0, stream>>>(kc, vc, ks, vs, pages, n, num_pages, kv_heads, block_bytes,
-                                                     static_cast<T*>(k_out), static_cast<T*>(v_out), scales);
+    read_kernel<T, kCodeE4M3><<<g, kReadThreads, 0, stream>>>(kc, vc, ks, vs, pages, n, num_pages, kv_heads,
+                                                              block_bytes, k, v, scales);
   }
   return cudaGetLastError();
 }

@@ -6,13 +6,16 @@
 // and the block scales stay outside the products.  The values' scale is
 // folded into the exponent,
 //
-//   u_j = log2(e) s_j,   n = running max u,   l = sum_j 2^(u_j - n)
-//   t_j = u_j + log2 vs_page(j),   m = running max t,   p_j = 2^(t_j - m)
+//   u_j = log2(e) s_j,                  l = sum_j 2^(u_j - n)
+//   t_j = u_j + log2 vs_page(j),        p_j = 2^(t_j - m)
 //   out = 2^(m - n) sum_j p_j c'_j / l
 //
-// so that p_j <= 1 is what the matrix unit multiplies the codes with,
-// whatever the blocks' scales are, and rounding p_j to fp16 is relative to
-// the largest contribution.  There is one exponential a token: within a block
+// so that p_j is what the matrix unit multiplies the codes with, whatever the
+// blocks' scales are, and rounding p_j to fp16 is relative to the largest
+// contribution.  m and n are references near the largest t and u: they are
+// set from the first tokens and raised, with what was summed so far brought
+// down, only where a weight passes kMostWeight, so that the ordinary step
+// looks for no maximum.  There is one exponential a token: within a block
 // 2^(u_j - n) is p_j times a number of the block.  Queries are brought to
 // |q| < 2 by a power of two of their own (exact), so fp16 holds bf16 queries
 // of any range.  m, n, l and the sums are fp32; l sums the unrounded p_j.
@@ -375,7 +378,7 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
         refill();
         continue;
       }
-      const float lv = value_exponent(vs, 0.0f, largest);
+      const float lv = value_exponent(vs, largest);
 
       // scores of tokens row_a and row_a + 8 (rows) for query rows 2t and
       // 2t + 1, in a chain of products for each piece of the key row

@@ -102,31 +102,43 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// Four codes (the bytes of w, in order) as fp16 operands.
+//
+// e4m3: every code is an fp16 number; the NaN byte is NaN, which append never
+// writes (a NaN or infinite token shows by its block's scale).
+//
 // int8 keys become operands without their sign: u = c + 128 in the low byte
 // of a half is the (subnormal) number u 2^-24, and the score is
 // q . u - 128 sum(q), a term of the row that the exponent's product takes in.
 // The sums do not cancel much: u is at most 255, twice the codes' spread.
-// Values are converted to c itself, whose sums may cancel to any degree.
-// Gain of the products over the codes' own.
-template <int CODE>
-__device__ __forceinline__ float key_gain() {
-  return CODE == kCodeInt8 ? 16777216.0f : 1.0f;
-}
-
-// Four codes -> four halves: keys (int8 as u 2^-24, see above) and values.
+//
+// int8 values are converted to c itself, since their weighted sums may cancel
+// to any degree: u below an exponent that makes it 1024 + u, minus 1152.
 template <int CODE, bool KEYS>
 __device__ __forceinline__ void to_operand(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if constexpr (CODE == kCodeE4M3) {
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
         : "=r"(lo), "=r"(hi)
         : "r"(w));
-  } else if constexpr (KEYS) {
-    const uint32_t u = w ^ 0x80808080u;
-    lo = __byte_perm(u, 0u, 0x4140);
-    hi = __byte_perm(u, 0u, 0x4342);
   } else {
-    codes_to_half<CODE>(w, lo, hi);
+    const uint32_t u = w ^ 0x80808080u, high = KEYS ? 0u : 0x64646464u;
+    lo = __byte_perm(u, high, 0x4140);
+    hi = __byte_perm(u, high, 0x4342);
+    if constexpr (!KEYS) {
+      const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
+      const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&lo), bias);
+      const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&hi), bias);
+      lo = *reinterpret_cast<const uint32_t*>(&x);
+      hi = *reinterpret_cast<const uint32_t*>(&y);
+    }
   }
+}
+
+// What the products with keys have to be multiplied by for it.
+template <int CODE>
+__device__ __forceinline__ float key_gain() {
+  return CODE == kCodeInt8 ? 16777216.0f : 1.0f;
 }
 
 // A block that no token was appended to may hold any scale: one at or below
@@ -136,8 +148,8 @@ __device__ __forceinline__ float value_scale(float s) { return s < kScaleFloor ?
 // log2 of a block's value scale, raised where it is 2^-64 of the largest one
 // that this warp has met: such a block's codes add nothing to the output, but
 // its p_j must not underflow, since the sum l still counts them.
-__device__ __forceinline__ float value_exponent(float scale, float gain_log2, float& largest) {
-  float lv = __log2f(value_scale(scale)) + gain_log2;
+__device__ __forceinline__ float value_exponent(float scale, float& largest) {
+  const float lv = __log2f(value_scale(scale));
   largest = fmaxf(largest, lv < 256.0f ? lv : largest);  // an infinite scale is a matter of its own block
   const float least = largest - 64.0f;
   return lv < least ? least : lv;

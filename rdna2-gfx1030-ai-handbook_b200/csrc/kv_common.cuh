@@ -230,35 +230,6 @@ __device__ __forceinline__ int warp_search(int batch, int64_t x, Key key) {
 }
 
 // ------------------------------------------------------------------ 8-bit codes
-// Four codes (the bytes of w, in order) -> two half2.  int8: u = c + 128 in
-// the low byte of a half whose exponent makes it 1024 + u, minus 1152.
-// e4m3: sign and magnitude moved to fp16's places give the value times 2^-8
-// (the exponent biases differ by 8), subnormals included; kCodeGain undoes
-// it in the block's scale.  The e4m3 NaN byte reads as 480: append writes a
-// block with a NaN or infinite token by its scale.
-template <int CODE>
-__device__ __forceinline__ float code_gain() {
-  return CODE == kCodeE4M3 ? 256.0f : 1.0f;
-}
-
-// The two bytes in the low halves of x's 16-bit fields -> two halves.
-template <int CODE>
-__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (CODE == kCodeInt8) {
-    const uint32_t u = w ^ 0x80808080u;
-    const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
-    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias);
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
-    lo = *reinterpret_cast<const uint32_t*>(&x);
-    hi = *reinterpret_cast<const uint32_t*>(&y);
-  } else {
-    const uint32_t a = __byte_perm(w, 0u, 0x1404), b = __byte_perm(w, 0u, 0x3424);
-    lo = (a & 0x80008000u) | ((a >> 1) & 0x3f803f80u);
-    hi = (b & 0x80008000u) | ((b >> 1) & 0x3f803f80u);
-  }
-}
-
 // Four codes of numbers x / scale, round to nearest even.  They are in the
 // codes' range but for a rounding, since the scale covers the block (adding
 // 1.5 * 2^23 leaves the integer in the low byte; e4m3 saturates).  Where the
@@ -279,10 +250,23 @@ __device__ __forceinline__ uint32_t pack_codes(const float (&x)[4], float scale)
   return scale < INFINITY ? w : 0u;
 }
 
+// The numbers that four codes stand for, before their scale: an int8 code +
+// 128 in the low byte of 2^23 + (c + 128), e4m3 by way of fp16.
 template <int CODE>
-__device__ __forceinline__ float from_code(uint32_t c) {
-  if constexpr (CODE == kCodeInt8) return static_cast<float>(static_cast<int8_t>(c));
-  return fp8_to_float(static_cast<uint8_t>(c), kE4M3);
+__device__ __forceinline__ void code_values(uint32_t w, float* f) {
+  if constexpr (CODE == kCodeInt8) {
+    const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7650 + j)) - 8388736.0f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> (16 * j)), __NV_E4M3);
+      const float2 v = __half22float2(__half2(h));
+      f[2 * j] = v.x;
+      f[2 * j + 1] = v.y;
+    }
+  }
 }
 
 }  // namespace b2

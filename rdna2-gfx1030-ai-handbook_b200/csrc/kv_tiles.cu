@@ -135,7 +135,7 @@ __device__ __forceinline__ bool load_block(const AttendParams& p, int slot, Bloc
   k.s = load_sequence(p, k.b);
   k.rows = k.s.count * p.group;
   k.row0 = (slot - first_block(p, k.b)) * kCtaRows;
-  if (k.row0 >= k.rows) return false;
+  if (k.row0 < 0 || k.row0 >= k.rows) return false;  // below 0: offsets that decrease
   int lo, hi, unused;
   const int last = min(k.row0 + kCtaRows, k.rows) - 1;
   row_bounds(p, k.s, k.s.start + k.row0 / p.group, lo, unused);

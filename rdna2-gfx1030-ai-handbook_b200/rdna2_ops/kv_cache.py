@@ -11,13 +11,17 @@ head), K and V apart; a value is code * scale.  The caller owns the paging:
 table[b, i] is the page of sequence b's tokens [i * page_size, (i + 1) *
 page_size), and lengths[b] counts its tokens, those of the call included.  A
 call's tokens are packed, [tokens, heads, head_dim]: the same number for every
-sequence, or rows offsets[b] .. offsets[b + 1]; the last one is at position
+sequence, or rows offsets[b] .. offsets[b + 1], with offsets[0] = 0 and the
+last one the number of tokens; a sequence's last row is at position
 lengths[b] - 1.  lengths, table and offsets are int32 on the device and are
 not read on the host: one lengths tensor serves every layer of a step.
 
 Tokens at negative positions, past the table, or on a table entry outside the
 cache (-1 marks an absent page) are not stored and not seen.  A page that a
-call appends to must belong to one sequence only.
+call appends to must belong to one sequence only.  Scales are not negative.
+The workspace of attend is kept for each stream, so one cache may serve calls
+on several; ordering its appends before the calls that read them is the
+caller's, as for any tensor.
 """
 from __future__ import annotations
 
@@ -39,11 +43,13 @@ HEAD_DIMS = (64, 128)
 def _rows(x):
     """x [tokens, heads, dim] itself where the kernels can read its rows (channels
     contiguous, rows at multiples of 16 bytes), else a copy."""
-    tokens, heads, dim = x.shape
-    step = 16 // x.element_size()
-    if x.stride(2) != 1 or x.stride(0) % step or x.stride(1) % step or x.data_ptr() % 16:
-        return x.clone(memory_format=torch.contiguous_format)
-    return x
+    if x.data_ptr() % 16 == 0:
+        if x.is_contiguous():
+            return x
+        step = 16 // x.element_size()
+        if x.stride(2) == 1 and x.stride(0) % step == 0 and x.stride(1) % step == 0:
+            return x
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 @functools.lru_cache(maxsize=1024)

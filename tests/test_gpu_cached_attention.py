@@ -62,6 +62,29 @@ def test_one_workspace_serves_calls_of_any_shape():
             first[tuple(counts)] = got[0]
 
 
+@pytest.mark.parametrize("offsets", [[0, 300, 100, 400], [50, 60, 70, 80], [0, -5, 1000, 7], [400, 0, 0, 0]])
+def test_offsets_that_make_no_sense_stay_inside(offsets):
+    """Decreasing, beyond the tokens, or not from 0: no result is promised, but
+    what lies around the outputs, the cache's other pages and its codes behind
+    them are as they were."""
+    lengths = [500, 30, 90]
+    table, pages = _paging(lengths, 32, random.Random(5))
+    cache = _filled(pages + 2, 2, 64, 32, "int8", seed=4)
+    used = set(table[table >= 0].tolist())
+    loose = torch.tensor([p for p in range(pages + 2) if p not in used]).cuda()
+    before = [t[loose].clone() for t in (cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale)]
+    off = torch.tensor(offsets, dtype=torch.int32).cuda()
+    lens, tab = torch.tensor(lengths, dtype=torch.int32).cuda(), table.cuda()
+    x = torch.randn(400, 6, 64, device="cuda").half()
+    for most in (1, 400):
+        out, lse = cache.attend(x, lens, tab, offsets=off, max_new=most, return_lse=True)
+        assert out.shape == x.shape and lse.shape == (400, 6)
+    cache.append(x[:, :2], x[:, 2:4], lens, tab, offsets=off)
+    torch.cuda.synchronize()
+    for a, t in zip(before, (cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale)):
+        assert torch.equal(a, t[loose])
+
+
 def _layer(window=None, code="int8"):
     from rdna2_ops.cached_attention import CachedAttention
     from rdna2_ops.convrot_checkpoint import quantize_convrot
