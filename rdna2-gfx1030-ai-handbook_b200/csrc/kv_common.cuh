@@ -113,14 +113,9 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // (a, b) -> (a cos - b sin, b cos + a sin), products and sums each rounded to
-// fp32 (no contraction), so the result is the same as elementwise torch.
+// fp32, so the result is the same as elementwise torch.  The intrinsics are
+// never contracted; a packed mul.rn.f32x2 and the add after it were.
 __device__ __forceinline__ void rotate_pair(float& a, float& b, float cos, float sin) {
   const float x = __fsub_rn(__fmul_rn(a, cos), __fmul_rn(b, sin));
   const float y = __fadd_rn(__fmul_rn(b, cos), __fmul_rn(a, sin));
@@ -163,12 +158,7 @@ __device__ __forceinline__ void rotate_unit(float (&a)[V], float (&b)[V], const 
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < V; i += 2) {  // rotate_pair for two pairs at once: b (-sin) is -(b sin)
-      const uint64_t x = pair_of(a[i], a[i + 1]), y = pair_of(b[i], b[i + 1]);
-      const uint64_t c = pair_of(cos[i], cos[i + 1]), s = pair_of(sin[i], sin[i + 1]);
-      unpair(add_pair(mul_pair(x, c), mul_pair(y, pair_of(-sin[i], -sin[i + 1]))), a[i], a[i + 1]);
-      unpair(add_pair(mul_pair(y, c), mul_pair(x, s)), b[i], b[i + 1]);
-    }
+    for (int i = 0; i < V; ++i) rotate_pair(a[i], b[i], cos[i], sin[i]);
   }
 }
 

@@ -346,6 +346,39 @@ def test_append(dtype, code, dim, page, rot, layout):
     _append(cache, counts, lengths, table, dtype, angles=angles, layout=layout, q_heads=1 if rot else 0, seed=9)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("layout,counts", [("half", [100, 33]), ("interleaved", [2, 1])])
+def test_append_bit_by_bit(dtype, code, layout, counts):
+    """Scales, codes and queries against the formulas in elementwise 32-bit torch."""
+    from rdna2_ops.kv_cache import PagedKVCache
+    from rdna2_ops.rotary import rope_table, rotary
+    cache = PagedKVCache(10, 3, 64, page_size=32, code=code)
+    table = torch.tensor([[4, 9, 0, 2], [7, 1, 3, 8]], dtype=torch.int32)
+    g = torch.Generator().manual_seed(2)
+    k, v, q = (torch.randn(sum(counts), n, 64, generator=g).to(dtype).cuda() for n in (3, 3, 5))
+    lengths, angles = torch.tensor(counts, dtype=torch.int32), rope_table(128, 64)
+    got = cache.append(k, v, lengths.cuda(), table.cuda(), offsets=_offsets(counts).cuda(), q=q, angles=angles,
+                       layout=layout)
+    where = places(lengths, _offsets(counts), sum(counts))
+    at = torch.tensor([p for _, p in where]).cuda()
+    assert torch.equal(got, rotary(q, angles, at, layout=layout))
+    top = torch.tensor(127.0 if code == "int8" else 448.0, device="cuda")
+    keys = rotary(k.float(), angles, at, layout=layout)  # held bit by bit to torch elsewhere
+    for x, codes, scales in ((keys, cache.k_codes, cache.k_scale), (v.float(), cache.v_codes, cache.v_scale)):
+        blocks = {}
+        for i, (b, pos) in enumerate(where):
+            blocks.setdefault(int(table[b, pos // 32]), []).append((i, pos % 32))
+        for page, rows in blocks.items():
+            new = x[[i for i, _ in rows]]
+            s = (new.abs().amax((0, 2)) / top).clamp_min(2.0 ** -100)
+            assert torch.equal(scales[page], s)
+            want = new * (1.0 / s)[:, None]
+            want = want.round().to(torch.int8) if code == "int8" else want.clamp(-top, top).to(torch.float8_e4m3fn)
+            held = codes.view(torch.uint8)[page][:, [slot for _, slot in rows]].transpose(0, 1)
+            assert torch.equal(held, want.view(torch.uint8))
+
+
 def test_append_skips_what_has_no_place():
     from rdna2_ops.kv_cache import PagedKVCache
     from rdna2_ops.rotary import rope_table
@@ -448,8 +481,9 @@ def test_refusals():
     ok = dict(lengths=lens, table=table)
     for exc, kw in [
             (TypeError, dict(q=x.float())), (ValueError, dict(q=x[:, :1])), (ValueError, dict(q=x[:3])),
-            (ValueError, dict(q=x[..., :32])), (TypeError, dict(lengths=lens.long())), (TypeError, dict(table=table.long())),
-            (ValueError, dict(lengths=lens[:1])), (ValueError, dict(table=table.t())), (ValueError, dict(offsets=off[:2])),
+            (ValueError, dict(q=x[..., :32])), (TypeError, dict(lengths=lens.long())),
+            (TypeError, dict(table=table.long())), (ValueError, dict(lengths=lens[:1])),
+            (ValueError, dict(table=table.t())), (ValueError, dict(offsets=off[:2])),
             (TypeError, dict(offsets=off.long())), (ValueError, dict(window=0)), (ValueError, dict(scale=0.0)),
             (ValueError, dict(scale=math.inf)), (ValueError, dict(lengths=lens.cpu())), (ValueError, dict(q=x.cpu())),
             (ValueError, dict(offsets=off, max_new=0)), (ValueError, dict(q=x.clone().requires_grad_()))]:
@@ -458,7 +492,8 @@ def test_refusals():
     angles = rope_table(8, 64)
     for exc, kw in [
             (TypeError, dict(k=x.int(), v=x.int())), (ValueError, dict(v=x.float())), (ValueError, dict(v=x[:, :1])),
-            (ValueError, dict(k=x[:, :1], v=x[:, :1])), (ValueError, dict(q=x)), (TypeError, dict(q=x.float(), angles=angles)),
+            (ValueError, dict(k=x[:, :1], v=x[:, :1])), (ValueError, dict(q=x)),
+            (TypeError, dict(q=x.float(), angles=angles)),
             (ValueError, dict(q=x[:2], angles=angles)), (ValueError, dict(angles=rope_table(8, 24))),
             (TypeError, dict(angles=angles.half())), (ValueError, dict(angles=angles, layout="other")),
             (ValueError, dict(offsets=off[:2])), (ValueError, dict(k=x[:3], v=x[:3]))]:

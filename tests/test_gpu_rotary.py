@@ -24,8 +24,8 @@ def _check(x, angles, positions, layout, inverse=False, **kw):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
 @pytest.mark.parametrize("tokens,heads,dim,rot", [
-    (1, 1, 2, 2), (1, 32, 128, 128), (3, 5, 64, 32), (37, 24, 128, 64), (7, 3, 80, 80), (5, 2, 96, 32), (2, 9, 256, 128),
-    (4, 3, 33, 10), (6, 1, 130, 128), (300, 17, 64, 64), (1, 1, 1024, 1000)])
+    (1, 1, 2, 2), (1, 32, 128, 128), (3, 5, 64, 32), (37, 24, 128, 64), (7, 3, 80, 80), (5, 2, 96, 32),
+    (2, 9, 256, 128), (4, 3, 33, 10), (6, 1, 130, 128), (300, 17, 64, 64), (1, 1, 1024, 1000)])
 def test_rotary(dtype, layout, tokens, heads, dim, rot):
     from rdna2_ops.rotary import rope_table
     g = torch.Generator().manual_seed(tokens * 1000 + dim)
@@ -34,6 +34,27 @@ def test_rotary(dtype, layout, tokens, heads, dim, rot):
     angles = rope_table(5000, rot)
     _check(x, angles, positions, layout)
     _check(x, angles, positions.int(), layout, inverse=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dim,rot", [(128, 128), (64, 32), (33, 10)])
+def test_bit_by_bit_with_elementwise_products_and_sums(dtype, layout, dim, rot):
+    """Every product and sum is rounded to fp32 on its own, in any layout."""
+    from rdna2_ops.rotary import rope_table, rotary
+    g = torch.Generator().manual_seed(dim)
+    x = torch.randn(500, 7, dim, generator=g).mul(20).to(dtype).cuda()
+    angles, positions = rope_table(3000, rot), torch.randint(0, 3000, (500,), generator=g).cuda()
+    row = angles[positions][:, None]
+    cos, sin = row[..., :rot // 2], row[..., rot // 2:]
+    f = x.float()
+    a, b = (f[..., :rot // 2], f[..., rot // 2:rot]) if layout == "half" else (f[..., 0:rot:2], f[..., 1:rot:2])
+    for inverse in (False, True):
+        s = -sin if inverse else sin
+        y, z = a * cos - b * s, b * cos + a * s
+        turned = torch.cat([y, z], -1) if layout == "half" else torch.stack([y, z], -1).flatten(-2)
+        want = torch.cat([turned, f[..., rot:]], -1).to(dtype)
+        assert torch.equal(rotary(x, angles, positions, layout=layout, inverse=inverse), want)
 
 
 def test_strided_in_place_and_out():
