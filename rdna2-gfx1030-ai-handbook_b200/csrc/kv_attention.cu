@@ -29,6 +29,11 @@
 // that keeps those reads free of bank conflicts.  Every warp has its own ring
 // of 16-token stages, filled by TMA, and its own softmax; the warps of a CTA,
 // and the CTAs that share a (sequence, kv head), are joined at its end.
+//
+// Memory should bound it and does not quite: about 410 instructions a warp for
+// 16 tokens of K and V, a third of them conversions.  One sequence of 262131
+// tokens, 8 kv heads of 128, 4 rows each, e4m3: 108 us for 537 MB, 5.0 TB/s;
+// 64 sequences of up to 8192, 8 rows each, int8: 120 us, 4.3 TB/s.
 #include "../../include/b2_attention.h"
 #include "b2_internal.h"
 #include "kv_attention.cuh"
