@@ -68,12 +68,13 @@ def rope_table(positions, rotary_dim, *, base=10000.0, scaling=None, factor=1.0,
 
 def angle_table(angles, dim, device):
     """Checks a table of angles for heads of `dim` channels."""
-    _args.require(isinstance(angles, torch.Tensor) and angles.dtype == torch.float32, TypeError,
-                  "angles must be an fp32 tensor")
-    _args.require(angles.ndim == 2 and angles.is_contiguous() and angles.device == device and angles.shape[0] >= 1,
-                  ValueError, f"angles must be contiguous [positions, rotary_dim] on {device}")
-    _args.require(angles.shape[1] >= 2 and angles.shape[1] % 2 == 0 and angles.shape[1] <= dim, ValueError,
-                  f"rotary_dim must be even and at most {dim}, got {angles.shape[1]}")
+    if not isinstance(angles, torch.Tensor) or angles.dtype != torch.float32:
+        raise TypeError("angles must be an fp32 tensor")
+    shape = angles.shape
+    if len(shape) != 2 or shape[0] < 1 or not angles.is_contiguous() or angles.device != device:
+        raise ValueError(f"angles must be contiguous [positions, rotary_dim] on {device}")
+    if shape[1] < 2 or shape[1] % 2 or shape[1] > dim:
+        raise ValueError(f"rotary_dim must be even and at most {dim}, got {shape[1]}")
 
 
 def rotary(x, angles, positions, *, layout="half", inverse=False, out=None):
