@@ -299,15 +299,20 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
       }
       __syncwarp();
     };
+    // The scores of a tile wait for its blocks' scales too, although only the
+    // softmax reads those: the warp that brings them goes by the parity of
+    // k_free, and would miss a phase if a second one could complete meanwhile.
     const int todo = t < used ? count : 0;
-    bool ok = todo == 0 || (wait(&ctl.q_full[t], 0, kSiteMma) && wait(&ctl.k_full[0], 0, kSiteMma));
+    bool ok = todo == 0 || (wait(&ctl.q_full[t], 0, kSiteMma) && wait(&ctl.k_full[0], 0, kSiteMma) &&
+                            wait(&ctl.info_full[0], 0, kSiteMma));
     if (ok && todo > 0) {
       tc_fence_after();
       scores(0);
     }
     for (int i = 0; ok && i < todo; ++i) {
       const auto next_scores = [&](uint64_t* before) {
-        ok = wait(&ctl.k_full[(i + 1) & 1], ((i + 1) >> 1) & 1, kSiteMma) && wait(before, i & 1, kSiteMma);
+        ok = wait(&ctl.k_full[(i + 1) & 1], ((i + 1) >> 1) & 1, kSiteMma) &&
+             wait(&ctl.info_full[(i + 1) & 3], ((i + 1) >> 2) & 1, kSiteMma) && wait(before, i & 1, kSiteMma);
         if (!ok) return;
         tc_fence_after();
         scores((i + 1) & 1);
@@ -328,8 +333,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
     __syncwarp();
   } else if (warp == kInfoWarp) {
     // ------------------------------------------------------- blocks' scales
-    // a lane a group of 16 tokens; the ring's place for tile i was last read
-    // by the softmax of tile i - 4, whose end the products of tile i - 2 need
+    // A lane a group of 16 tokens.  The ring's place for tile i was last read
+    // by the softmax of tile i - 4, whose end the scores of tile i - 2 need:
+    // they have been formed when k_free completes its phase, and the next phase
+    // needs the scores of tile i, which wait for what is written here.
     int64_t block = lane < kGroups ? block_of(token0 + 16 * lane) : -1;
     float ks = 0.0f, vs = 0.0f, largest = -INFINITY;
     const auto load = [&] {
