@@ -11,14 +11,18 @@
 //   out = 2^(m - n) sum_j p_j c'_j / l
 //
 // so that p_j is what the matrix unit multiplies the codes with, whatever the
-// blocks' scales are, and rounding p_j to fp16 is relative to the largest
-// contribution.  m and n are references near the largest t and u: they are
+// blocks' scales are.  p_j is rounded to fp16 for it, by 2^-12 of itself or
+// 2^-31 of the largest one: products of 32-bit weights would take twice the
+// matrix unit's time or more, and outputs of 16 bits would not show them (fp16
+// outputs are off by 2.1e-4 to 2.4e-4 from 64 bits, 2.05e-4 with 32-bit
+// weights).  m and n are references near the largest t and u: they are
 // set from the first tokens and raised, with what was summed so far brought
 // down, only where a weight passes kMostWeight, so that the ordinary step
 // looks for no maximum.  There is one exponential a token: within a block
 // 2^(u_j - n) is p_j times a number of the block.  Queries are brought to
-// |q| < 2 by a power of two of their own (exact), so fp16 holds bf16 queries
-// of any range.  m, n, l and the sums are fp32; l sums the unrounded p_j.
+// |q| < 2 by a power of two of their own, so fp16 holds bf16 queries of any
+// range: exactly, but for channels below 2^-14 of a row's largest, which may be
+// off by 2^-25 of it.  m, n, l and the sums are fp32; l sums the unrounded p_j.
 //
 // kv_rows_kernel: few query rows.  The rows of one kv head (its query heads
 // times the call's tokens) are the N = 8 or 16 columns of mma.sync m16n8k16
@@ -442,7 +446,7 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
             float top = fmaxf(sc[n][col], sc[n][col + 2]);
 #pragma unroll
             for (int s = 4; s < kWarp; s *= 2) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, s));
-            const float next = fmaxf(m[n][col], top), next_u = fmaxf(mu[n][col], top - lv);
+            const float next = fmaxf(m[n][col], top - kReferenceLog2), next_u = fmaxf(mu[n][col], top - lv);
             const float ref = next == -INFINITY ? 0.0f : next, alpha = weight_of(m[n][col], next);
             l[n][col] *= weight_of(mu[n][col], next_u);
             m[n][col] = next;

@@ -49,12 +49,6 @@ constexpr int kTilesThreads = 28 * kWarp;
 // Registers a thread: 72 at launch, 4 * 80 + 2 * 64 + 56 = 7 * 72 afterwards.
 constexpr int kSoftmaxRegs = 80, kConvertRegs = 64, kOtherRegs = 56;
 constexpr int kHalfTokens = kTileTokens / 2;  // of a softmax thread
-// A reference is set this far above the tile's maximum.  Together with
-// kMostWeight it leaves 2^20 for what later tiles bring: going through a tile
-// twice costs as much as a tile, and with 2^13 a prompt whose keys are
-// unequally loud did so in every fourth of its first tiles.  Weights below
-// 2^-9 of the largest are subnormal fp16 then, off by 2^-20 of it at most.
-constexpr float kHeadroomLog2 = 5.0f;
 constexpr uint32_t kMinusInf = 0xff800000u;
 
 // One row tile of queries, or one tile of K or V: panels of 64 channels, 128
@@ -580,7 +574,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
           ctl.row[0][half][cta_row] = top_t;
           ctl.row[1][half][cta_row] = top_u;
           named_bar_sync(pair, 2 * kWarp);
-          const float next = fmaxf(m, fmaxf(top_t, ctl.row[0][other][cta_row]) + kHeadroomLog2);
+          const float next = fmaxf(m, fmaxf(top_t, ctl.row[0][other][cta_row]) - kReferenceLog2);
           const float next_n = fmaxf(ctl.n[me], fmaxf(top_u, ctl.row[1][other][cta_row]));
           const float alpha = weight_of(m, next);
           ctl.l[me] *= weight_of(ctl.n[me], next_n);

@@ -1,11 +1,15 @@
-"""Attention over the cache where its kernels' pipelines could go wrong: long
-walks over the cache."""
+"""Attention over the cache against 64 bits, with bounds that follow from its
+arithmetic term by term, and where its kernels' pipelines could go wrong."""
+import math
 import random
 
 import pytest
 import torch
 
-from test_gpu_kv_cache import _filled, _offsets, _paging
+from kv_reference import assert_close, places
+from test_gpu_kv_cache import _filled, _offsets, _paging, _values
+
+from conftest import GAMMA_FP32
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +46,101 @@ def test_long_walks_repeat_themselves(dim, page, count):
         for _ in range(10):
             again = _run(cache, q, [count], [length], table)
             assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+# ------------------------------------------------------------ 64 bits, bounds
+TOP = {"int8": 127.0, "e4m3": 448.0}
+
+
+def _exact(cache, q, counts, lengths, table, causal=True, window=None, scale=None, only=None):
+    """(out, lse, bound of out, bound of lse) in 64 bits, of the heads `only`
+    or all, and the pages that each row sees.
+
+    With w_j the softmax of a row and R the largest w_j vs_j in it:
+
+    * A score's products are exact and summed in fp32, GAMMA_FP32 of the sum of
+      their magnitudes, int8 keys as c + 128; a query channel below fp16's
+      normal numbers is off by 2^-25 of the row's largest.  The exponent, its
+      argument and the logarithms add 2^-20: e in all, relative to w_j and
+      absolute in the log-sum-exp.
+    * A weight that multiplies a code is fp16: off by 2^-11 of itself or, below
+      fp16's normal numbers, by 2^-25 of its unit, where the largest is
+      2^6 units at least, so by 2^-31 R / vs_j.
+    """
+    k, v = _values(cache)
+    vs, ks = cache.v_scale.cpu().double(), cache.k_scale.cpu().double()
+    tokens, heads, dim = q.shape
+    group, page = heads // k.shape[1], k.shape[2]
+    scale = dim ** -0.5 if scale is None else scale
+    q = q.cpu().double()
+    out, lse = torch.zeros_like(q), torch.full((tokens, heads), -math.inf, dtype=torch.float64)
+    out_tol, lse_tol, seen = torch.zeros_like(q), torch.zeros(tokens, heads, dtype=torch.float64), []
+    for i, (b, pos) in enumerate(places(torch.tensor(lengths), _offsets(counts), tokens)):
+        hi = min(lengths[b], table.shape[1] * page)
+        at = torch.arange(max(0, pos - window + 1) if window else 0, max(0, min(hi, pos + 1) if causal else hi))
+        pid = table[b, at // page].long()
+        at, pid = at[pid >= 0], pid[pid >= 0]
+        seen.append(set(pid.tolist()))
+        if not len(at):
+            continue
+        for h in range(heads) if only is None else only:
+            g = h // group
+            kk, vv, units = k[pid, g, at % page], v[pid, g, at % page], vs[pid, g].clamp_min(2.0 ** -100)
+            s = kk @ q[i, h] * scale
+            size = kk.abs() @ q[i, h].abs() + q[i, h].abs().sum() * 128 * ks[pid, g] * (cache.code == "int8")
+            e = ((GAMMA_FP32 * size + 2.0 ** -25 * q[i, h].abs().max() * kk.abs().sum(1)) * scale).max() + 2.0 ** -20
+            lse[i, h] = torch.logsumexp(s, 0)
+            w = torch.exp(s - lse[i, h])
+            out[i, h] = w @ vv
+            out_tol[i, h] = (2.0 ** -11 + 4 * e) * (w @ vv.abs()) + 2.0 ** -31 * (w * units).max() * (
+                vv.abs() / units[:, None]).sum(0)
+            lse_tol[i, h] = 2 * e + 2.0 ** -22 * lse[i, h].abs()
+    return out, lse, out_tol, lse_tol, seen
+
+
+def _check(cache, q, counts, lengths, table, only=None, **kw):
+    want = _exact(cache, q, counts, lengths, table, only=only, **kw)
+    out, lse = _run(cache, q, counts, lengths, table, **kw)
+    some = list(range(q.shape[1])) if only is None else only
+    assert_close(out[:, some], want[0][:, some], want[2][:, some], q.dtype, "out")
+    assert_close(lse[:, some], want[1][:, some], want[3][:, some], torch.float32, "lse")
+
+
+def _queries(counts, heads, dim, dtype=torch.float16, seed=0):
+    return torch.randn(sum(counts), heads, dim, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("code,dtype", [("int8", torch.float16), ("e4m3", torch.float16), ("int8", torch.bfloat16)])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 32), (64, 128), (128, 64)])
+@pytest.mark.parametrize("counts", [[1, 4], [60, 33]])
+@pytest.mark.parametrize("kw", [{}, dict(window=77), dict(causal=False)])
+def test_within_the_bounds(code, dtype, dim, page, counts, kw):
+    lengths = [700, 333]
+    table, pages = _paging(lengths, page, random.Random(dim + page))
+    cache = _filled(pages, 2, dim, page, code, seed=page)
+    _check(cache, _queries(counts, 6, dim, dtype), counts, lengths, table, **kw)
+
+
+# ------------------------------------------------------ many small weights
+@pytest.mark.parametrize("code,dim", [("int8", 64), ("int8", 128), ("e4m3", 64), ("e4m3", 128)])
+@pytest.mark.parametrize("count,heads,length", [(1, 1, 8192), (40, 1, 8192), (1, 300, 1024), (40, 160, 512)])
+@pytest.mark.parametrize("log2", [-12, -20, -22, -26])
+@pytest.mark.parametrize("last", [False, True])
+def test_many_small_weights_beside_a_large_one(code, dim, count, heads, length, log2, last):
+    """One token takes nearly all of the weight and has no value; many others,
+    2^log2 of it each, are all that comes out.  With many heads a CTA walks the
+    whole of a history."""
+    lengths = [length + count]
+    at = length - 2 if last else 0
+    table, pages = _paging(lengths, 64, random.Random(2))
+    cache = _filled(pages, heads, dim, 64, code, seed=4)
+    cache.k_codes.view(torch.uint8).zero_()
+    cache.v_scale.fill_(0.01)
+    cache.k_scale.fill_(0.125)
+    sink = int(table[0, at // 64])
+    # a score of -log2 * ln 2 for queries of one channel: scale * q * code * ks
+    cache.k_codes[sink, :, at % 64, 0] = 64
+    cache.v_codes.view(torch.uint8)[sink, :, at % 64] = 0
+    q = torch.zeros(count, heads, dim)
+    q[..., 0] = -log2 * math.log(2) / (8.0 * dim ** -0.5)
+    _check(cache, q.half().cuda(), [count], lengths, table, only=[0, heads - 1])
