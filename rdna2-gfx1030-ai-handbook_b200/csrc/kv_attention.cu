@@ -461,13 +461,15 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
           }
       }
       uint32_t pf[NT][2];
+      // a row that sees a block with a NaN scale has NaN weights; one that does not has zeros, and must not meet it
+      const float lw = lv != lv ? 0.0f : lv;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int col = 0; col < 2; ++col) {
           const float ref = m[n][col] == -INFINITY ? 0.0f : m[n][col];
           const float ref_u = mu[n][col] == -INFINITY ? 0.0f : mu[n][col];
-          l[n][col] = fmaf(weight[n][col] + weight[n][col + 2], exp2_approx(ref - lv - ref_u), l[n][col]);
+          l[n][col] = fmaf(weight[n][col] + weight[n][col + 2], exp2_approx(ref - lw - ref_u), l[n][col]);
         }
         pf[n][0] = transpose_8x8(pack_half2(weight[n][0], weight[n][1]));
         pf[n][1] = transpose_8x8(pack_half2(weight[n][2], weight[n][3]));

@@ -546,6 +546,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
         a = product * key_gain<CODE>();
         a = a == 0.0f ? 1.17549435e-38f : a;
       };
+      // Whether this row sees none of a block's tokens here: their scores are
+      // -inf, and the block's scales, which may be no numbers, must not meet them.
+      const auto hidden = [&](int x) {
+        const int at = base + x * SEG;
+        return max(ctl.lo[me], at) >= min(ctl.hi[me], at + SEG) || !(present >> (x * (SEG / 16)) & 1);
+      };
       ok = ok && wait(&ctl.s_full[tile], i & 1, kSiteEpilogue);
       if (used == 2 && i + tile > 0) ok = ok && wait(&ctl.turn[tile], (i + tile - 1) & 1, kSiteEpilogue);
       tc_fence_after();
@@ -601,10 +607,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
         uint32_t sc[32];
 #pragma unroll
         for (int x = 0; x < kHalfTokens / SEG; ++x) {
-          const GroupInfo g = info[x * (SEG / 16)];
+          GroupInfo g = info[x * (SEG / 16)];
           float a, d;
           factor(g, a, d);
           d += g.lv - ref;
+          if (!whole && hidden(x)) a = 1.0f, d = -INFINITY, g.iv = 0.0f;
           const uint64_t aa = pair_of(a, a), dd = pair_of(d, d);
           uint64_t part = 0;
 #pragma unroll

@@ -144,3 +144,47 @@ def test_many_small_weights_beside_a_large_one(code, dim, count, heads, length, 
     q = torch.zeros(count, heads, dim)
     q[..., 0] = -log2 * math.log(2) / (8.0 * dim ** -0.5)
     _check(cache, q.half().cuda(), [count], lengths, table, only=[0, heads - 1])
+
+
+# ----------------------------------------------- masked blocks of no numbers
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("code,dim,page", [("int8", 64, 16), ("e4m3", 128, 16), ("e4m3", 64, 32), ("int8", 128, 32),
+                                           ("int8", 128, 64), ("e4m3", 64, 64)])
+@pytest.mark.parametrize("counts,kw", [([8], {}), ([8], dict(window=3)), ([4], dict(window=8, causal=False)),
+                                       ([12], {}), ([12], dict(window=5)),
+                                       ([180], {}), ([180], dict(window=20)), ([300], dict(window=40, causal=False))])
+def test_a_block_of_no_numbers_shows_in_the_rows_that_see_it_alone(bad, which, code, dim, page, counts, kw):
+    """As an append of a NaN or an infinity leaves it: its scale is no number
+    and its codes are 0.  Rows on earlier pages, and rows whose window begins
+    behind it, are as if it were any other block."""
+    lengths = [324 if counts == [8] else 330]
+    table, pages = _paging(lengths, page, random.Random(page))
+    cache = _filled(pages, 2, dim, page, code, seed=dim)
+    odd = int(table[0, (lengths[0] - counts[0] // 2) // page - (1 if kw else 0)])
+    for codes in (cache.k_codes, cache.v_codes):
+        codes.view(torch.uint8)[odd] = 0
+    q = _queries(counts, 4, dim)
+    want = _exact(cache, q, counts, lengths, table, **kw)
+    getattr(cache, which)[odd, 1] = bad  # of the second kv head
+    out, lse = _run(cache, q, counts, lengths, table, **kw)
+    sees = torch.tensor([[odd in s and h >= 2 for h in range(4)] for s in want[4]])
+    assert sees.any() and not sees[:, 2:].all()
+    assert not torch.isfinite(out[sees.cuda()]).any()
+    assert_close(out[~sees.cuda()], want[0][~sees], want[2][~sees], q.dtype, "out")
+    assert_close(lse[~sees.cuda()], want[1][~sees], want[3][~sees], torch.float32, "lse")
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("counts", [[3], [100]])
+def test_a_row_that_sees_nothing_of_no_numbers_is_zero(bad, counts):
+    """Positions below zero, with a query or the only block of no numbers."""
+    lengths = [2]
+    table, pages = _paging(lengths, 16, random.Random(1))
+    cache = _filled(pages, 1, 64, 16, "int8", seed=1)
+    cache.k_scale[int(table[0, 0])] = cache.v_scale[int(table[0, 0])] = bad
+    q = _queries(counts, 2, 64)
+    q[0, 1, 7] = bad
+    out, lse = _run(cache, q, counts, lengths, table)
+    assert not out[:counts[0] - 2].any() and (lse[:counts[0] - 2] == -math.inf).all()
+    assert not torch.isfinite(out[counts[0] - 2:]).any()
