@@ -387,7 +387,8 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
         refill();
         continue;
       }
-      const float lv = value_exponent(vs, largest);
+      bool quiet;
+      const float lv = value_exponent(vs, largest, quiet);
 
       // scores of tokens row_a and row_a + 8 (rows) for query rows 2t and
       // 2t + 1, in a chain of products for each piece of the key row
@@ -416,8 +417,8 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
       const bool whole = lo_most <= base && base + 16 <= hi_least;
       // t of the group's tokens, their weights against the references of
       // earlier groups, and whether those have to be raised: a row has none
-      // yet, or a weight is above what fp16 should hold
-      bool raise = false;
+      // yet, or a weight is above what fp16 should hold, or the block is quiet
+      bool raise = quiet;
       float weight[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -469,7 +470,11 @@ __global__ void __launch_bounds__(kRowsThreads, NT == 1 ? 2 : 1)
         for (int col = 0; col < 2; ++col) {
           const float ref = m[n][col] == -INFINITY ? 0.0f : m[n][col];
           const float ref_u = mu[n][col] == -INFINITY ? 0.0f : mu[n][col];
-          l[n][col] = fmaf(weight[n][col] + weight[n][col + 2], exp2_approx(ref - lw - ref_u), l[n][col]);
+          if (quiet) {
+            l[n][col] += exp2_approx(sc[n][col] - lv - ref_u) + exp2_approx(sc[n][col + 2] - lv - ref_u);
+          } else {
+            l[n][col] = fmaf(weight[n][col] + weight[n][col + 2], exp2_approx(ref - lw - ref_u), l[n][col]);
+          }
         }
         pf[n][0] = transpose_8x8(pack_half2(weight[n][0], weight[n][1]));
         pf[n][1] = transpose_8x8(pack_half2(weight[n][2], weight[n][3]));

@@ -17,10 +17,10 @@ constexpr float kMostWeight = 49152.0f;
 // weights down to 2^-(24 + kReferenceLog2) of that one.  Those below half of
 // that round to zero, while the sum of the weights, in fp32, counts them: over
 // 2^18 tokens up to 2^-13 of the largest weight is lost with 6, and a quarter
-// of it would be with a reference 2^5 above the largest.  What lies between here and kMostWeight is what later tokens may bring before
-// the reference is raised, which the tile kernel pays for with a second pass
-// over a tile: an 8192-token prompt takes 698 us with 6, 690, 683 and 676 us
-// with 3, 0 and -5.
+// of it would be with a reference 2^5 above the largest.  What lies between
+// here and kMostWeight is what later tokens may bring before the reference is
+// raised, which the tile kernel pays for with a second pass over a tile: an
+// 8192-token prompt takes 698 us with 6, 690, 683 and 676 us with 3, 0 and -5.
 constexpr float kReferenceLog2 = 6.0f;
 
 struct AttendParams {
@@ -155,14 +155,20 @@ __device__ __forceinline__ float key_gain() {
 // zero has no logarithm and reads as the smallest scale.  NaN stays NaN.
 __device__ __forceinline__ float value_scale(float s) { return s < kScaleFloor ? kScaleFloor : s; }
 
-// log2 of a block's value scale, raised where it is 2^-64 of the largest one
-// that this warp has met: such a block's codes add nothing to the output, but
-// its p_j must not underflow, since the sum l still counts them.
-__device__ __forceinline__ float value_exponent(float scale, float& largest) {
+// Quiet blocks.  A token's share of l is its p_j divided by its block's value
+// scale, which holds while p_j does not underflow where 2^(u_j - n) counts:
+// m is at most n + the largest log2 vs met, so a block within 2^-kQuietLog2 of
+// that one has its p_j above 2^-70 there.  A block below it is quiet: its share
+// of l is summed from exponentials of its own, against a raised n.
+constexpr float kQuietLog2 = 64.0f;
+
+// log2 of a block's value scale, and whether the block is quiet beside the
+// largest scale that this warp has met.
+__device__ __forceinline__ float value_exponent(float scale, float& largest, bool& quiet) {
   const float lv = __log2f(value_scale(scale));
   largest = fmaxf(largest, lv < 256.0f ? lv : largest);  // an infinite scale is a matter of its own block
-  const float least = largest - 64.0f;
-  return lv < least ? least : lv;
+  quiet = lv < largest - kQuietLog2;
+  return lv;
 }
 
 // Two running sums are joined relative to the larger maximum; a side that has

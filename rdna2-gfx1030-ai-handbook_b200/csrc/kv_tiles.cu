@@ -55,6 +55,8 @@ constexpr uint32_t kMinusInf = 0xff800000u;
 // rows of 128 bytes each, 128-byte swizzle.
 constexpr int kPanel = 128 * 128;
 
+constexpr uint32_t kQuiet = 1u << kGroups;
+
 struct __align__(16) GroupInfo {
   float ks, lv, iv, unused;  // key scale, log2 of the value scale, 2^(top_lv - lv)
 };
@@ -96,7 +98,10 @@ struct TilesControl {
   uint64_t s_full[2], s_read[2], p_full[2], o_done[2], info_full[4], turn[2], last[2];
   GroupInfo info[4][kGroups];
   float top_lv[4];
-  uint32_t present[4];  // bit g: group g lies on a page of the cache
+  // bit g: group g lies on a page of the cache; kQuiet, for each half of the
+  // tokens: the tile has a quiet block, its weights are summed apart, and iv is
+  // 0 and top_lv infinite
+  uint32_t present[4];
   Work work;
   // what the two threads of a row tell each other: maxima, and the sum of q
   float row[2][2][kCtaRows], sum[2][kCtaRows];
@@ -340,22 +345,21 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
     load();
     for (int i = 0; i < count; ++i) {
       const bool here = block >= 0;
-      float lv = here ? __log2f(value_scale(vs)) : -INFINITY;
+      const float lv = here ? __log2f(value_scale(vs)) : -INFINITY;
       float top = lv < 256.0f ? lv : -INFINITY;
 #pragma unroll
       for (int d = 1; d < kGroups; d *= 2) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
       top = __shfl_sync(kFullMask, top, 0);
       largest = fmaxf(largest, top);
-      if (here && lv < largest - 64.0f) lv = largest - 64.0f;
-      const float ref = fmaxf(top, largest - 64.0f);
-      const unsigned present = __ballot_sync(kFullMask, here);
-      const GroupInfo info = {ks, lv, here ? exp2_approx(ref - lv) : 0.0f, 0.0f};
+      const bool quiet = __any_sync(kFullMask, here && lv < largest - kQuietLog2);
+      const unsigned present = __ballot_sync(kFullMask, here) | (quiet ? kQuiet | kQuiet << kGroups / 2 : 0u);
+      const GroupInfo info = {ks, lv, here && !quiet ? exp2_approx(top - lv) : 0.0f, 0.0f};
       block = lane < kGroups && i + 1 < count ? block_of(token0 + (i + 1) * kTileTokens + 16 * lane) : -1;
       load();
       if (i >= 2 && !wait(&ctl.k_free[i & 1], ((i >> 1) & 1) ^ 1, kSiteTransform)) break;
       if (lane < kGroups) ctl.info[i & 3][lane] = info;
       if (lane == 0) {
-        ctl.top_lv[i & 3] = ref == -INFINITY ? 0.0f : ref;
+        ctl.top_lv[i & 3] = quiet ? INFINITY : top == -INFINITY ? 0.0f : top;
         ctl.present[i & 3] = present;
       }
       __syncwarp();
@@ -546,18 +550,19 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
         a = product * key_gain<CODE>();
         a = a == 0.0f ? 1.17549435e-38f : a;
       };
-      // Whether this row sees none of a block's tokens here: their scores are
-      // -inf, and the block's scales, which may be no numbers, must not meet them.
-      const auto hidden = [&](int x) {
-        const int at = base + x * SEG;
-        return max(ctl.lo[me], at) >= min(ctl.hi[me], at + SEG) || !(present >> (x * (SEG / 16)) & 1);
+      // Whether this row sees none of the `tokens` from group g on, which are one
+      // block's: their scores are -inf, and the block's scales, which may be no
+      // numbers, must not meet them.
+      const auto hidden = [&](int g, int tokens) {
+        const int at = base + g * 16;
+        return max(ctl.lo[me], at) >= min(ctl.hi[me], at + tokens) || !(present >> g & 1);
       };
       ok = ok && wait(&ctl.s_full[tile], i & 1, kSiteEpilogue);
       if (used == 2 && i + tile > 0) ok = ok && wait(&ctl.turn[tile], (i + tile - 1) & 1, kSiteEpilogue);
       tc_fence_after();
       uint32_t w[kHalfTokens / 2];
       float sum, ref;
-      bool raise = i == 0, last = true;  // last: the turn has not been passed on
+      bool raise = i == 0 || present & kQuiet, last = true;  // last: the turn has not been passed on
       for (;;) {
         if (raise) {
           float top_t = -INFINITY, top_u = -INFINITY;
@@ -600,6 +605,25 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
               tmem_st32(o_col + 32 * c, o);
             }
           }
+          if (present & kQuiet) {
+            const float from = next_n == -INFINITY ? 0.0f : next_n;
+            float all = 0.0f;
+#pragma unroll 1
+            for (int c = 0; c < kHalfTokens / 32; ++c) {
+              uint32_t sc[32];
+              fetch(c, sc);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                float a, d;
+                factor(info[2 * c + h], a, d);
+                d -= from;
+                if (!whole && hidden(2 * c + h, 16)) a = 1.0f, d = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) all += exp2_approx(fmaf(__uint_as_float(sc[16 * h + j]), a, d));
+              }
+            }
+            ctl.l[me] += all;
+          }
         }
         ref = m == -INFINITY ? 0.0f : m;
         float weights = 0.0f;
@@ -611,7 +635,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
           float a, d;
           factor(g, a, d);
           d += g.lv - ref;
-          if (!whole && hidden(x)) a = 1.0f, d = -INFINITY, g.iv = 0.0f;
+          if (!whole && hidden(x * (SEG / 16), SEG)) a = 1.0f, d = -INFINITY, g.iv = 0.0f;
           const uint64_t aa = pair_of(a, a), dd = pair_of(d, d);
           uint64_t part = 0;
 #pragma unroll

@@ -188,3 +188,36 @@ def test_a_row_that_sees_nothing_of_no_numbers_is_zero(bad, counts):
     out, lse = _run(cache, q, counts, lengths, table)
     assert not out[:counts[0] - 2].any() and (lse[:counts[0] - 2] == -math.inf).all()
     assert not torch.isfinite(out[counts[0] - 2:]).any()
+
+
+# ------------------------------------------------------- value scales far apart
+@pytest.mark.parametrize("counts,page", [([2], 16), ([2], 64), ([100], 16), ([100], 128)])
+@pytest.mark.parametrize("order", [1, -1])
+@pytest.mark.parametrize("apart", [2.0 ** -30, 2.0 ** -64, 2.0 ** -70, 2.0 ** -90])
+@pytest.mark.parametrize("hide", ["score", "window", "none"])
+def test_quiet_blocks_that_the_softmax_favours(counts, page, order, apart, hide):
+    """Blocks whose values are `apart` of the others', where those have next to
+    no weight, or are hidden: the quiet values come out as they are, whichever
+    blocks come first."""
+    blocks, dim = 512 // page, 64
+    lengths = [512]
+    table, pages = _paging(lengths, page, random.Random(page))
+    cache = _filled(pages, 1, dim, page, "int8", seed=3, spread=0.1)
+    row = table[0].long().cuda()
+    late = torch.arange(blocks).cuda() * page >= 256  # the last 256 tokens
+    quiet = row[late if order == 1 else ~late]
+    loud = row[~late if order == 1 else late]
+    cache.v_scale[loud], cache.v_scale[quiet] = 0.25, 0.25 * apart
+    kw = {}
+    q = _queries(counts, 2, dim, torch.bfloat16)
+    if hide == "score":  # about -150 for the loud ones
+        q = q * 0.05 + 18.75
+        cache.k_codes[loud] = -100
+        cache.k_scale[loud] = 0.01
+        cache.k_codes[quiet] //= 16
+    elif hide == "window" and order == 1:
+        kw = dict(window=256 if counts == [2] else 200)  # the last rows see quiet ones alone
+    elif hide == "window":  # every row ends in the quiet half
+        lengths = [250]
+    q = q.bfloat16()
+    _check(cache, q, counts, lengths, table, **kw)
