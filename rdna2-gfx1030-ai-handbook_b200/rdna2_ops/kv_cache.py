@@ -44,11 +44,11 @@ def _rows(x):
     """x [tokens, heads, dim] itself where the kernels can read its rows (channels
     contiguous, rows at multiples of 16 bytes), else a copy."""
     if x.data_ptr() % 16 == 0:
-        if x.is_contiguous():
-            return x
         step = 16 // x.element_size()
         if x.stride(2) == 1 and x.stride(0) % step == 0 and x.stride(1) % step == 0:
             return x
+        if x.is_contiguous():  # the stride of a dimension of one entry is anything
+            return x.as_strided(x.shape, (x.shape[1] * x.shape[2], x.shape[2], 1))
     return x.clone(memory_format=torch.contiguous_format)
 
 
