@@ -17,7 +17,8 @@
  * table[b][0 .. width), position p on page table[b][p / page].  The call's
  * tokens are packed; sequence b has rows offsets[b] .. offsets[b + 1], or
  * tokens / batch rows each where offsets is NULL, and its last row is at
- * position lengths[b] - 1.  Table entries outside [0, pages) hold no tokens.
+ * position lengths[b] - 1.  Table entries outside [0, pages) hold no tokens;
+ * a cache of no pages needs no memory.
  */
 #ifndef B2_ATTENTION_H_
 #define B2_ATTENTION_H_

@@ -402,7 +402,8 @@ int b2_kv_append(const void* k, const void* v, int dtype, int64_t tokens, int64_
   if (pages < 0 || pages > INT32_MAX) return invalid;
   if (tokens == 0) return 0;
   if (batch < 1 || (offsets == nullptr && tokens % batch)) return invalid;
-  if (!k || !v || !lengths || (!table && width) || !k_codes || !v_codes || !k_scale || !v_scale) return invalid;
+  if (!k || !v || !lengths || (!table && width)) return invalid;
+  if (pages && (!k_codes || !v_codes || !k_scale || !v_scale)) return invalid;
   const int64_t unit = dtype == b2::kF32 ? 4 : 8;
   const auto rows_ok = [&](const void* x, int64_t ts, int64_t hs) {
     return b2::aligned16(x) && ts >= 0 && hs >= 0 && ts % unit == 0 && hs % unit == 0;
@@ -460,7 +461,8 @@ int b2_kv_read(const void* k_codes, const void* v_codes, const float* k_scale, c
     return invalid;
   if ((dim != 64 && dim != 128) || (page != 16 && page != 32 && page != 64 && page != 128)) return invalid;
   if (n == 0) return 0;
-  if (!k_codes || !v_codes || !k_scale || !v_scale || !pages || !k_out || !v_out) return invalid;
+  if (num_pages && (!k_codes || !v_codes || !k_scale || !v_scale)) return invalid;
+  if (!pages || !k_out || !v_out) return invalid;
   if (!b2::aligned16(k_codes) || !b2::aligned16(v_codes) || !b2::aligned16(k_out) || !b2::aligned16(v_out))
     return invalid;
   const auto* kc = static_cast<const uint8_t*>(k_codes);

@@ -758,7 +758,8 @@ int b2_kv_attention(const void* q, int dtype, int64_t tokens, int64_t q_heads, i
   if (pages < 0 || pages * kv_heads > INT32_MAX || window < 0 || !(scale > 0.0f) || scale > 3.0e38f) return invalid;
   if (tokens == 0) return 0;
   if (batch < 1 || max_new < 1 || (offsets == nullptr && (tokens % batch || tokens / batch > max_new))) return invalid;
-  if (!q || !lengths || (!table && width) || !k_codes || !v_codes || !k_scale || !v_scale || !out) return invalid;
+  if (!q || !lengths || (!table && width) || !out) return invalid;
+  if (pages && (!k_codes || !v_codes || !k_scale || !v_scale)) return invalid;
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(k_codes, 16) || !aligned(v_codes, 16)) return invalid;
   if (q_token_stride < 0 || q_head_stride < 0 || q_token_stride % 8 || q_head_stride % 8) return invalid;
   const b2::Plan plan = b2::make_plan(tokens, batch, max_new, q_heads, kv_heads, dim, width, page, window);
