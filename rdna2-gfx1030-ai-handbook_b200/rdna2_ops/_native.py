@@ -7,6 +7,7 @@ device is missing.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -146,6 +147,22 @@ def check(status, what):
     if status != 0:
         msg = library().b2_error_string(status)
         raise RuntimeError(f"{what} failed: {msg.decode() if msg else status}")
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device):
+    """A context in which `device` is the current one."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def launch(device, name, *args):
+    """Calls the C entry point `name` with `args` and the current stream of
+    `device`.  The device is made the current one for it: a kernel is launched
+    there, on whichever device its tensors lie (a default stream names none)."""
+    with on_device(device):
+        check(getattr(library(), name)(*args, stream_ptr(device)), name)
 
 
 def ptr(t):

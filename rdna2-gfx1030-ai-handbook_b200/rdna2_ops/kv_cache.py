@@ -53,8 +53,9 @@ def _rows(x):
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_bytes(*shape):
-    return nat.library().b2_kv_attention_workspace_bytes(*shape)
+def _workspace_bytes(device, *shape):
+    with nat.on_device(device):
+        return nat.library().b2_kv_attention_workspace_bytes(*shape)
 
 
 class PagedKVCache:
@@ -165,12 +166,12 @@ class PagedKVCache:
         if tokens == 0:
             return rotated
         k, v = _rows(k), _rows(v)
-        nat.check(nat.library().b2_kv_append(
-            k.data_ptr(), v.data_ptr(), nat.DTYPE_CODE[k.dtype], tokens, self.kv_heads, self.head_dim, k.stride(0),
-            k.stride(1), v.stride(0), v.stride(1), lengths.data_ptr(), nat.ptr(offsets), batch, table.data_ptr(), width,
-            nat.ptr(q), 0 if q is None else q.shape[1], 0 if q is None else q.stride(0),
-            0 if q is None else q.stride(1), nat.ptr(rotated), nat.ptr(angles), rows, rotary_dim, LAYOUTS[layout],
-            _CODE_INDEX[self.k_codes.dtype], *self._memory(), self.page_size, nat.stream_ptr(dev)), "b2_kv_append")
+        nat.launch(
+            dev, "b2_kv_append", k.data_ptr(), v.data_ptr(), nat.DTYPE_CODE[k.dtype], tokens, self.kv_heads,
+            self.head_dim, k.stride(0), k.stride(1), v.stride(0), v.stride(1), lengths.data_ptr(), nat.ptr(offsets),
+            batch, table.data_ptr(), width, nat.ptr(q), 0 if q is None else q.shape[1],
+            0 if q is None else q.stride(0), 0 if q is None else q.stride(1), nat.ptr(rotated), nat.ptr(angles), rows,
+            rotary_dim, LAYOUTS[layout], _CODE_INDEX[self.k_codes.dtype], *self._memory(), self.page_size)
         return rotated
 
     # ---------------------------------------------------------------- attend
@@ -209,17 +210,17 @@ class PagedKVCache:
         lse = torch.empty((tokens, heads), device=dev, dtype=torch.float32) if return_lse else None
         if tokens:
             q = _rows(q)
-            lib, stream = nat.library(), nat.stream_ptr(dev)
-            need = _workspace_bytes(tokens, batch, max_new, heads, self.kv_heads, self.head_dim, width,
+            stream = nat.stream_ptr(dev)
+            need = _workspace_bytes(dev, tokens, batch, max_new, heads, self.kv_heads, self.head_dim, width,
                                     self.page_size, window or 0)
             work = self._workspaces.get(stream)
             if work is None or work.numel() < need:
                 work = self._workspaces[stream] = torch.zeros(need, device=dev, dtype=torch.uint8)
-            nat.check(lib.b2_kv_attention(
-                q.data_ptr(), nat.DTYPE_CODE[q.dtype], tokens, heads, q.stride(0), q.stride(1), lengths.data_ptr(),
-                nat.ptr(offsets), batch, max_new, table.data_ptr(), width, _CODE_INDEX[self.k_codes.dtype],
-                *self._memory(), self.kv_heads, self.page_size, self.head_dim, scale, int(causal), window or 0,
-                out.data_ptr(), nat.ptr(lse), work.data_ptr(), work.numel(), stream), "b2_kv_attention")
+            nat.launch(
+                dev, "b2_kv_attention", q.data_ptr(), nat.DTYPE_CODE[q.dtype], tokens, heads, q.stride(0), q.stride(1),
+                lengths.data_ptr(), nat.ptr(offsets), batch, max_new, table.data_ptr(), width,
+                _CODE_INDEX[self.k_codes.dtype], *self._memory(), self.kv_heads, self.page_size, self.head_dim, scale,
+                int(causal), window or 0, out.data_ptr(), nat.ptr(lse), work.data_ptr(), work.numel())
         return (out, lse) if return_lse else out
 
     # ------------------------------------------------------------------ read
@@ -238,8 +239,8 @@ class PagedKVCache:
         shape = (pages.shape[0], self.kv_heads, self.page_size, self.head_dim)
         k, v = torch.empty(shape, device=dev, dtype=dtype), torch.empty(shape, device=dev, dtype=dtype)
         scales = torch.empty((2, *shape[:2]), device=dev, dtype=torch.float32) if return_scales else None
-        nat.check(nat.library().b2_kv_read(
-            *self._memory()[:4], _CODE_INDEX[self.k_codes.dtype], self.num_pages, self.kv_heads, self.page_size,
-            self.head_dim, pages.data_ptr(), shape[0], nat.DTYPE_CODE[dtype], k.data_ptr(), v.data_ptr(),
-            nat.ptr(scales), nat.stream_ptr(dev)), "b2_kv_read")
+        nat.launch(
+            dev, "b2_kv_read", *self._memory()[:4], _CODE_INDEX[self.k_codes.dtype], self.num_pages, self.kv_heads,
+            self.page_size, self.head_dim, pages.data_ptr(), shape[0], nat.DTYPE_CODE[dtype], k.data_ptr(),
+            v.data_ptr(), nat.ptr(scales))
         return (k, v, *scales.unbind()) if return_scales else (k, v)

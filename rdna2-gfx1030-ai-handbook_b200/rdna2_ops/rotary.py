@@ -105,9 +105,8 @@ def rotary(x, angles, positions, *, layout="half", inverse=False, out=None):
         raise ValueError("out must have x's shape, type and device, and contiguous channels")
     if x.stride(2) != 1:
         x = x.contiguous()
-    nat.check(nat.library().b2_rotary(
-        x.data_ptr(), nat.DTYPE_CODE[x.dtype], tokens, heads, dim, x.stride(0), x.stride(1), angles.data_ptr(),
-        angles.shape[0], angles.shape[1], LAYOUTS[layout], int(inverse), positions.data_ptr(),
-        int(positions.dtype == torch.int64), out.data_ptr(), out.stride(0), out.stride(1), nat.stream_ptr(dev)),
-        "b2_rotary")
+    nat.launch(
+        dev, "b2_rotary", x.data_ptr(), nat.DTYPE_CODE[x.dtype], tokens, heads, dim, x.stride(0), x.stride(1),
+        angles.data_ptr(), angles.shape[0], angles.shape[1], LAYOUTS[layout], int(inverse), positions.data_ptr(),
+        int(positions.dtype == torch.int64), out.data_ptr(), out.stride(0), out.stride(1))
     return out
