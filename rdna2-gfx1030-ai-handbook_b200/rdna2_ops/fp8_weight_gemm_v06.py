@@ -50,9 +50,10 @@ def decode_fp8_weight(w, *, out_dtype=torch.float16, metadata=None):
     if w.stride(1) != 1:
         w = w.contiguous()
     out = torch.empty((n, k), dtype=out_dtype, device=w.device)
-    nat.check(nat.library().b2_fp8_decode(
+    nat.launch(
+        w.device, "b2_fp8_decode",
         w.data_ptr(), nat.DTYPE_CODE[w.dtype], n, k, w.stride(0) if n > 1 else k,
-        nat.DTYPE_CODE[out_dtype], out.data_ptr(), k, nat.stream_ptr(w.device)), "b2_fp8_decode")
+        nat.DTYPE_CODE[out_dtype], out.data_ptr(), k)
     if metadata is not None:
         metadata.update(method="software_decode", output_dtype=str(out_dtype),
                         kernel="fp8_decode_kernel")
@@ -66,9 +67,10 @@ def _quant_rows(x):
         x = x.contiguous()
     q = torch.empty((m, k), dtype=torch.int8, device=x.device)
     s = torch.empty(m, dtype=torch.float32, device=x.device)
-    nat.check(nat.library().b2_act_quant(
+    nat.launch(
+        x.device, "b2_act_quant",
         x.data_ptr(), nat.DTYPE_CODE[x.dtype], m, k, x.stride(0) if m > 1 else k, 0, 2, q.data_ptr(),
-        k, s.data_ptr(), nat.stream_ptr(x.device)), "b2_act_quant")
+        k, s.data_ptr())
     return q, s
 
 

@@ -192,10 +192,11 @@ def pack_int4(w, *, group_size=64, symmetric=True, layout="nk", order="low"):
     scales = torch.empty((n, k // group_size), device=dev, dtype=torch.float32)
     zeros = torch.empty_like(scales, dtype=torch.int32)
     sums = torch.empty_like(zeros)
-    nat.check(nat.library().b2_pack_int4(
+    nat.launch(
+        dev, "b2_pack_int4",
         w.data_ptr(), nat.DTYPE_CODE[w.dtype], w.stride(0) if n > 1 else k, n, k, group_size,
         int(bool(symmetric)), int(layout == "kn"), int(order == "high"), data.data_ptr(),
-        scales.data_ptr(), zeros.data_ptr(), sums.data_ptr(), nat.stream_ptr(dev)), "b2_pack_int4")
+        scales.data_ptr(), zeros.data_ptr(), sums.data_ptr())
     return PackedInt4(data, scales, zeros, sums, n, k, group_size, bool(symmetric), layout, order)
 
 
@@ -206,10 +207,10 @@ def unpack_int4(p, *, dtype=torch.float16):
         raise TypeError(dtype)
     out = torch.empty((p.n, p.k), device=p.data.device, dtype=dtype)
     code = {torch.float32: nat.F32, torch.float16: nat.F16, torch.int8: 3}[dtype]
-    nat.check(nat.library().b2_unpack_int4(
+    nat.launch(
+        p.data.device, "b2_unpack_int4",
         p.data.data_ptr(), int(p.layout == "kn"), int(p.order == "high"), p.scales.data_ptr(),
-        p.zeros.data_ptr(), p.n, p.k, p.group_size, code, out.data_ptr(),
-        nat.stream_ptr(p.data.device)), "b2_unpack_int4")
+        p.zeros.data_ptr(), p.n, p.k, p.group_size, code, out.data_ptr())
     return out
 
 
@@ -226,10 +227,11 @@ def prepare_w4a16(p, dtype=torch.bfloat16):
     groups = torch.empty((t, p.k // p.group_size, 128), device=p.data.device, dtype=torch.int32)
     assert tiles.numel() * 4 == lib.b2_w4a16_tiles_bytes(p.n, p.k)
     assert groups.numel() * 4 == lib.b2_w4a16_groups_bytes(p.n, p.k, p.group_size)
-    nat.check(lib.b2_w4a16_prepare(
+    nat.launch(
+        p.data.device, "b2_w4a16_prepare",
         p.data.data_ptr(), int(p.layout == "kn"), int(p.order == "high"), p.scales.data_ptr(),
         p.zeros.data_ptr(), p.n, p.k, p.group_size, nat.DTYPE_CODE[dtype], tiles.data_ptr(),
-        groups.data_ptr(), nat.stream_ptr(p.data.device)), "b2_w4a16_prepare")
+        groups.data_ptr())
     return W4A16Weight(tiles, groups, p.n, p.k, p.group_size, dtype, source_stamp(p))
 
 
@@ -265,11 +267,12 @@ def w4a16_gemm(a, wt, bias=None, *, workspace=None):
     if need and (workspace is None or workspace.numel() < need):
         # arrival counters at the end must start at zero; calls keep them zero
         workspace = torch.zeros(need, device=dev, dtype=torch.uint8)
-    nat.check(lib.b2_w4a16_gemm(
+    nat.launch(
+        dev, "b2_w4a16_gemm",
         a.data_ptr(), nat.DTYPE_CODE[a.dtype], a.stride(0) if m > 1 else wt.k, wt.tiles.data_ptr(),
         wt.groups.data_ptr(), wt.group_size, m, wt.n, wt.k, nat.ptr(bias),
         nat.DTYPE_CODE[bias.dtype] if bias is not None else 0, out.data_ptr(), wt.n,
-        None if not need else workspace.data_ptr(), need, nat.stream_ptr(dev)), "b2_w4a16_gemm")
+        None if not need else workspace.data_ptr(), need)
     return out
 
 
@@ -341,10 +344,10 @@ def prepare_w4a8(p):
     tiles = torch.empty(lib.b2_w4a8_tiles_bytes(p.n, p.k), device=p.data.device, dtype=torch.uint8)
     groups = torch.empty(lib.b2_w4a8_groups_bytes(p.n, p.k, p.group_size), device=p.data.device,
                          dtype=torch.uint8)
-    nat.check(lib.b2_w4a8_prepare(
+    nat.launch(
+        p.data.device, "b2_w4a8_prepare",
         p.data.data_ptr(), int(p.layout == "kn"), int(p.order == "high"), p.scales.data_ptr(),
-        p.zeros.data_ptr(), p.n, p.k, p.group_size, tiles.data_ptr(), groups.data_ptr(),
-        nat.stream_ptr(p.data.device)), "b2_w4a8_prepare")
+        p.zeros.data_ptr(), p.n, p.k, p.group_size, tiles.data_ptr(), groups.data_ptr())
     return W4A8Weight(tiles, groups, p.n, p.k, p.group_size, source_stamp(p))
 
 
@@ -406,10 +409,10 @@ def int4_linear_a8(a, p, a_scale, *, bias=None, method="dot4", tile=(64, 64), nu
     need = lib.b2_w4a8_workspace_bytes(m, k, wt.group_size)
     ws = torch.empty(max(need, 256), device=dev, dtype=torch.uint8)
     sa = a_scale.reshape(-1) if a_scale is not None else None
-    nat.check(lib.b2_w4a8_gemm(
+    nat.launch(
+        dev, "b2_w4a8_gemm",
         a.data_ptr(), a.stride(0) if m > 1 else k, wt.tiles.data_ptr(), wt.groups.data_ptr(), wt.group_size,
         m, n, k, nat.ptr(sa), nat.ptr(bias), nat.DTYPE_CODE[bias.dtype] if bias is not None else 0,
-        int(bool(integer)), out.data_ptr(), n, ws.data_ptr(), ws.numel(), nat.stream_ptr(dev)),
-        "b2_w4a8_gemm")
+        int(bool(integer)), out.data_ptr(), n, ws.data_ptr(), ws.numel())
     kernel = {"name": "w4a8_kernel (tcgen05 kind::i8, swap-AB, per-group TMEM drain)", "arch": "sm_100a"}
     return (out, kernel) if return_kernel else out

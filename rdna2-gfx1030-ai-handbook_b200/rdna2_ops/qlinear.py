@@ -100,10 +100,10 @@ def act_quant(x, *, rotation_block=None, quant="int8", out=None, scale=None):
     if m == 0:
         return out, scale
     ldx = x2.stride(0) if m > 1 else k
-    nat.check(nat.library().b2_act_quant(
+    nat.launch(
+        dev, "b2_act_quant",
         x2.data_ptr(), nat.DTYPE_CODE[x.dtype], m, k, ldx, block, 0 if quant == "int8" else 1,
-        out.data_ptr(), out.stride(0) if m > 1 else k, scale.data_ptr(), nat.stream_ptr(dev)),
-        "b2_act_quant")
+        out.data_ptr(), out.stride(0) if m > 1 else k, scale.data_ptr())
     return out, scale
 
 
@@ -132,8 +132,8 @@ def _kmajor(t, elem_bytes, s_row, s_col, rows, cols):
     ld = _round_up(max(cols, 1), 16 // elem_bytes)
     dtype = torch.uint8 if elem_bytes == 1 else torch.int16
     buf = torch.empty((rows, ld), device=t.device, dtype=dtype)
-    nat.check(nat.library().b2_repack(t.data_ptr(), elem_bytes, rows, cols, s_row, s_col,
-                                      buf.data_ptr(), ld, nat.stream_ptr(t.device)), "b2_repack")
+    nat.launch(t.device, "b2_repack", t.data_ptr(), elem_bytes, rows, cols, s_row, s_col,
+               buf.data_ptr(), ld)
     return buf, ld
 
 
@@ -158,11 +158,11 @@ def qgemm_raw(kind, a, w, a_scale, w_scale, bias, epilogue, out):
         w_t, ldw = op if op else _kmajor(w, eb, w.stride(0), w.stride(1), n, k)
     out_code = nat.DTYPE_CODE[out.dtype]
     bias_code = nat.DTYPE_CODE[bias.dtype] if bias is not None else 0
-    nat.check(nat.library().b2_qgemm(
+    nat.launch(
+        dev, "b2_qgemm",
         kind, a_t.data_ptr(), lda, w_t.data_ptr(), ldw, m, n, k, nat.ptr(a_scale),
         nat.ptr(w_scale), 0 if w_scale is None else w_scale.numel(), nat.ptr(bias), bias_code,
-        epilogue, out.data_ptr(), out_code, out.stride(0) if m > 1 else n,
-        nat.stream_ptr(dev)), "b2_qgemm")
+        epilogue, out.data_ptr(), out_code, out.stride(0) if m > 1 else n)
     return out
 
 
@@ -203,12 +203,13 @@ def w8a8_linear(x, w_q, w_scale, bias=None, *, rotation_block=None, out_dtype=No
     need = lib.b2_quant_linear_workspace_bytes(m, k)
     if workspace is None or workspace.numel() < need:
         workspace = torch.empty(need, device=dev, dtype=torch.uint8)
-    nat.check(lib.b2_quant_linear(
+    nat.launch(
+        dev, "b2_quant_linear",
         nat.KIND_I8 if kind == "int8" else nat.KIND_E4M3, x2.data_ptr(), nat.DTYPE_CODE[x.dtype], m,
         k, x2.stride(0) if m > 1 else k, block, w_t.data_ptr(), ldw, n, w_scale.data_ptr(),
         w_scale.numel(), nat.ptr(bias), nat.DTYPE_CODE[bias.dtype] if bias is not None else 0,
         EPILOGUES[epilogue], out.data_ptr(), nat.DTYPE_CODE[out_dtype], n, workspace.data_ptr(),
-        workspace.numel(), nat.stream_ptr(dev)), "b2_quant_linear")
+        workspace.numel())
     return out.reshape(*x.shape[:-1], n)
 
 

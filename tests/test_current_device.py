@@ -51,8 +51,8 @@ def notes(request, monkeypatch):
     before = notes.current
     yield notes
     assert notes.current == before
-    assert notes.calls and all(call[1] == 1 for call in notes.calls), notes.calls
-    assert all(call[2] == 1001 for call in notes.calls if not call[0].endswith("bytes")), notes.calls
+    launches = [call for call in notes.calls if not call[0].endswith("bytes")]
+    assert launches and all(call[1:] == (1, 1001) for call in launches), notes.calls
 
 
 def _names(notes):
@@ -84,3 +84,22 @@ def test_attend_and_read(notes):
     cache.read(table[0])
     kv_cache._workspace_bytes.cache_clear()
     assert _names(notes) == ["b2_kv_attention_workspace_bytes", "b2_kv_attention", "b2_kv_read"]
+    assert notes.calls[0][1] == 1  # it goes by the device's multiprocessors
+
+
+def test_quantized_linears(notes, monkeypatch):
+    from rdna2_ops import _args, qlinear
+    monkeypatch.setattr(_args, "fp32_vector", lambda *args, **kw: None)  # would compare devices
+    w = torch.zeros(32, 64, dtype=torch.int8)
+    qlinear.act_quant(torch.zeros(2, 64))
+    qlinear.w8a8_linear(torch.zeros(2, 64), w, torch.ones(32))
+    assert [n for n in _names(notes) if not n.endswith("bytes")] == ["b2_act_quant", "b2_quant_linear"]
+
+
+def test_every_launch_goes_by_its_device():
+    """No wrapper takes a stream by itself, but those of a process that has one device."""
+    from conftest import PKG
+    for path in sorted((PKG / "rdna2_ops").glob("*.py")):
+        if path.name not in ("_native.py", "column_parallel.py"):
+            text = path.read_text().replace("stream = nat.stream_ptr(dev)", "")  # a workspace's key
+            assert "stream_ptr" not in text, path.name
