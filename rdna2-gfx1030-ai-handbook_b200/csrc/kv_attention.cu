@@ -704,6 +704,7 @@ Plan make_plan(int64_t tokens, int64_t batch, int64_t max_new, int64_t q_heads, 
                int64_t width, int64_t page, int64_t window) {
   Plan plan{};
   const int64_t group = q_heads / kv_heads;
+  if (max_new > tokens) max_new = tokens;
   plan.tiles = max_new * group > kRowsMost;
   if (plan.tiles) {
     plan.workspace = kRowsMaxGrid * sizeof(int) + tiles_workspace_bytes(tokens, batch, group, kv_heads,
