@@ -724,6 +724,9 @@ Plan make_plan(int64_t tokens, int64_t batch, int64_t max_new, int64_t q_heads, 
   return plan;
 }
 
+// A window of 2^31 tokens reaches over any sequence.
+int64_t held_window(int64_t window) { return window < (int64_t(1) << 31) ? window : int64_t(1) << 31; }
+
 bool shapes_ok(int64_t tokens, int64_t batch, int64_t max_new, int64_t q_heads, int64_t kv_heads, int64_t dim,
                int64_t width, int64_t page) {
   if (tokens < 0 || tokens > INT32_MAX / 2 || batch < 0 || batch > (1 << 20) || max_new < 0) return false;
@@ -743,7 +746,7 @@ size_t b2_kv_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t ma
   if (!b2::shapes_ok(tokens, batch, max_new, q_heads, kv_heads, dim, width, page) || window < 0 || tokens == 0 ||
       batch == 0)
     return 0;
-  return b2::make_plan(tokens, batch, max_new, q_heads, kv_heads, dim, width, page, window).workspace;
+  return b2::make_plan(tokens, batch, max_new, q_heads, kv_heads, dim, width, page, b2::held_window(window)).workspace;
 }
 
 int b2_kv_attention(const void* q, int dtype, int64_t tokens, int64_t q_heads, int64_t q_token_stride,
@@ -763,6 +766,7 @@ int b2_kv_attention(const void* q, int dtype, int64_t tokens, int64_t q_heads, i
   if (pages && (!k_codes || !v_codes || !k_scale || !v_scale)) return invalid;
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(k_codes, 16) || !aligned(v_codes, 16)) return invalid;
   if (q_token_stride < 0 || q_head_stride < 0 || q_token_stride % 8 || q_head_stride % 8) return invalid;
+  window = b2::held_window(window);
   const b2::Plan plan = b2::make_plan(tokens, batch, max_new, q_heads, kv_heads, dim, width, page, window);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < plan.workspace) return invalid;
   b2::AttendParams p{};

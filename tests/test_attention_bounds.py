@@ -1,5 +1,9 @@
-"""Bounds far beyond any sequence mean what a large enough one means."""
+"""Windows and bounds on new tokens far beyond any sequence mean what a large
+enough one means."""
+import random
+
 import pytest
+import torch
 
 import rdna2_ops._native as nat
 
@@ -10,3 +14,22 @@ def test_workspaces(most):
     for heads, window in ((8, 0), (32, 0), (32, 100)):
         want = need(400, 2, 400, heads, 8, 128, 64, 64, window)
         assert want > 0 and need(400, 2, most, heads, 8, 128, 64, 64, window) == want
+    assert need(400, 2, 400, 32, 8, 128, 64, 64, max(most, 2 ** 20)) == need(400, 2, 400, 32, 8, 128, 64, 64, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 62, 2 ** 63 - 1])
+@pytest.mark.parametrize("counts", [[7, 3], [60, 30]])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_window_over_everything(window, counts, causal):
+    from test_gpu_kv_cache import _filled, _offsets, _paging
+    lengths = [counts[0] - 5, 100]  # five rows at positions below zero
+    table, pages = _paging(lengths, 16, random.Random(1))
+    cache = _filled(pages, 2, 64, 16, "int8", seed=1)
+    q = torch.randn(sum(counts), 4, 64, generator=torch.Generator().manual_seed(1)).half().cuda()
+    args = q, torch.tensor(lengths, dtype=torch.int32).cuda(), table.cuda()
+    off = _offsets(counts).cuda()
+    for most in (max(counts), window):
+        want = cache.attend(*args, offsets=off, causal=causal, max_new=min(most, sum(counts)), return_lse=True)
+        got = cache.attend(*args, offsets=off, causal=causal, window=window, max_new=most, return_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
