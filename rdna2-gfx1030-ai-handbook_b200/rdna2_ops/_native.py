@@ -149,20 +149,20 @@ def check(status, what):
         raise RuntimeError(f"{what} failed: {msg.decode() if msg else status}")
 
 
-_HERE = contextlib.nullcontext()
-
-
 def on_device(device):
     """A context in which `device` is the current one."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def launch(device, name, *args):
     """Calls the C entry point `name` with `args` and the current stream of
     `device`.  The device is made the current one for it: a kernel is launched
     there, on whichever device its tensors lie (a default stream names none)."""
-    with on_device(device):
+    if device.index == torch.cuda.current_device():
         check(getattr(library(), name)(*args, stream_ptr(device)), name)
+    else:
+        with torch.cuda.device(device):
+            check(getattr(library(), name)(*args, stream_ptr(device)), name)
 
 
 def ptr(t):
