@@ -50,12 +50,14 @@ constexpr int kTilesThreads = 28 * kWarp;
 constexpr int kSoftmaxRegs = 80, kConvertRegs = 64, kOtherRegs = 56;
 constexpr int kHalfTokens = kTileTokens / 2;  // of a softmax thread
 constexpr uint32_t kMinusInf = 0xff800000u;
+constexpr float kMostOffset = 2.59614843e33f;  // 2^111: a row's bias is below 2^17
 
 // One row tile of queries, or one tile of K or V: panels of 64 channels, 128
 // rows of 128 bytes each, 128-byte swizzle.
 constexpr int kPanel = 128 * 128;
 
 constexpr uint32_t kQuiet = 1u << kGroups;
+constexpr int kOddBit = 2 * kGroups;
 
 struct __align__(16) GroupInfo {
   float ks, lv, iv, unused;  // key scale, log2 of the value scale, 2^(top_lv - lv)
@@ -98,9 +100,11 @@ struct TilesControl {
   uint64_t s_full[2], s_read[2], p_full[2], o_done[2], info_full[4], turn[2], last[2];
   GroupInfo info[4][kGroups];
   float top_lv[4];
-  // bit g: group g lies on a page of the cache; kQuiet, for each half of the
-  // tokens: the tile has a quiet block, its weights are summed apart, and iv is
-  // 0 and top_lv infinite
+  // Bit g: group g lies on a page of the cache and has scales that are numbers.
+  // Bit kOddBit + g: it has scales that are not.  It is masked then, so that
+  // they meet no row that does not see it, and the sum of the weights of the
+  // rows that do is NaN.  kQuiet, for each half of the tokens: the tile has a
+  // quiet block, its weights are summed apart, and iv is 0 and top_lv infinite.
   uint32_t present[4];
   Work work;
   // what the two threads of a row tell each other: maxima, and the sum of q
@@ -344,16 +348,17 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
     };
     load();
     for (int i = 0; i < count; ++i) {
-      const bool here = block >= 0;
+      const bool odd = block >= 0 && !(fabsf(ks) < INFINITY && fabsf(vs) < INFINITY), here = block >= 0 && !odd;
       const float lv = here ? __log2f(value_scale(vs)) : -INFINITY;
-      float top = lv < 256.0f ? lv : -INFINITY;
+      float top = lv;
 #pragma unroll
       for (int d = 1; d < kGroups; d *= 2) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, d));
       top = __shfl_sync(kFullMask, top, 0);
       largest = fmaxf(largest, top);
       const bool quiet = __any_sync(kFullMask, here && lv < largest - kQuietLog2);
-      const unsigned present = __ballot_sync(kFullMask, here) | (quiet ? kQuiet | kQuiet << kGroups / 2 : 0u);
-      const GroupInfo info = {ks, lv, here && !quiet ? exp2_approx(top - lv) : 0.0f, 0.0f};
+      const unsigned present = __ballot_sync(kFullMask, here) | (quiet ? kQuiet | kQuiet << kGroups / 2 : 0u) |
+                               __ballot_sync(kFullMask, odd) << kOddBit;
+      const GroupInfo info = {here ? ks : 0.0f, lv, here && !quiet ? exp2_approx(top - lv) : 0.0f, 0.0f};
       block = lane < kGroups && i + 1 < count ? block_of(token0 + (i + 1) * kTileTokens + 16 * lane) : -1;
       load();
       if (i >= 2 && !wait(&ctl.k_free[i & 1], ((i >> 1) & 1) ^ 1, kSiteTransform)) break;
@@ -518,8 +523,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
       ctl.hi[me] = hi;
       ctl.n[me] = m;
       ctl.l[me] = 0.0f;
-      // what int8 keys without their sign add to a row's products
-      ctl.bias[me] = CODE == kCodeInt8 ? -128.0f * (ctl.sum[0][cta_row] + ctl.sum[1][cta_row]) : 0.0f;
+      // what int8 keys without their sign add to a row's products; those are no
+      // numbers where this is none, and masked ones must not become so
+      const float sum = ctl.sum[0][cta_row] + ctl.sum[1][cta_row];
+      ctl.bias[me] = CODE == kCodeInt8 && fabsf(sum) < INFINITY ? -128.0f * sum : 0.0f;
     }
     bool ok = true;
     for (int i = 0; i < count; ++i) {
@@ -532,6 +539,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
       // every row of this warp sees every one of its tokens
       const bool whole = __all_sync(kFullMask, ctl.lo[me] <= base && base + kHalfTokens <= ctl.hi[me]) &&
                          (present & 0xfu) == 0xfu;
+      if (!whole && present >> kOddBit & 0xfu) {
+#pragma unroll 1
+        for (int g = 0; g < kHalfTokens / 16; ++g)
+          if (present >> (kOddBit + g) & 1 && max(ctl.lo[me], base + 16 * g) < min(ctl.hi[me], base + 16 * g + 16))
+            ctl.l[me] = __int_as_float(0x7fffffff);
+      }
 
       // 32 scores; -inf where masked
       const auto fetch = [&](int c, uint32_t (&x)[32]) {
@@ -543,19 +556,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
         for (int j = 0; j < 32; ++j) x[j] = seen >> j & 1 ? x[j] : kMinusInf;
       };
       // Factor and offset that make u of a product, for one block.  A factor
-      // of zero would make NaN of a masked score.
+      // of zero, or an infinite offset, would make NaN of a masked score.
       const auto factor = [&](const GroupInfo& g, float& a, float& d) {
         const float product = qs * g.ks;
-        d = ctl.bias[me] * product;
+        d = ctl.bias[me] * fminf(product, kMostOffset);
         a = product * key_gain<CODE>();
         a = a == 0.0f ? 1.17549435e-38f : a;
-      };
-      // Whether this row sees none of the `tokens` from group g on, which are one
-      // block's: their scores are -inf, and the block's scales, which may be no
-      // numbers, must not meet them.
-      const auto hidden = [&](int g, int tokens) {
-        const int at = base + g * 16;
-        return max(ctl.lo[me], at) >= min(ctl.hi[me], at + tokens) || !(present >> g & 1);
       };
       ok = ok && wait(&ctl.s_full[tile], i & 1, kSiteEpilogue);
       if (used == 2 && i + tile > 0) ok = ok && wait(&ctl.turn[tile], (i + tile - 1) & 1, kSiteEpilogue);
@@ -617,7 +623,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
                 float a, d;
                 factor(info[2 * c + h], a, d);
                 d -= from;
-                if (!whole && hidden(2 * c + h, 16)) a = 1.0f, d = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < 16; ++j) all += exp2_approx(fmaf(__uint_as_float(sc[16 * h + j]), a, d));
               }
@@ -631,11 +636,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) kv_tiles_kernel(TilesParams 
         uint32_t sc[32];
 #pragma unroll
         for (int x = 0; x < kHalfTokens / SEG; ++x) {
-          GroupInfo g = info[x * (SEG / 16)];
+          const GroupInfo g = info[x * (SEG / 16)];
           float a, d;
           factor(g, a, d);
           d += g.lv - ref;
-          if (!whole && hidden(x * (SEG / 16), SEG)) a = 1.0f, d = -INFINITY, g.iv = 0.0f;
           const uint64_t aa = pair_of(a, a), dd = pair_of(d, d);
           uint64_t part = 0;
 #pragma unroll

@@ -190,6 +190,26 @@ def test_a_row_that_sees_nothing_of_no_numbers_is_zero(bad, counts):
     assert not torch.isfinite(out[counts[0] - 2:]).any()
 
 
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("counts", [[8], [12], [150]])
+def test_a_masked_block_that_would_overflow_stays_masked(code, counts):
+    """Queries near 1e30 over keys near 1e-30, and, where it is masked, a block
+    whose scores would be infinite."""
+    lengths, page = [324], 16
+    table, pages = _paging(lengths, page, random.Random(3))
+    cache = _filled(pages, 1, 64, page, code, seed=6)
+    cache.k_scale.mul_(1e-30)
+    q = (_queries(counts, 2, 64).float() * 1e30).bfloat16()
+    odd = int(table[0, lengths[0] // page])
+    want = _exact(cache, q, counts, lengths, table)
+    cache.k_scale[odd] = 1e20
+    out, lse = _run(cache, q, counts, lengths, table)
+    free = torch.tensor([odd not in s for s in want[4]])
+    assert free.any() and not free.all()
+    assert_close(out[free.cuda()], want[0][free], want[2][free], q.dtype, "out")
+    assert_close(lse[free.cuda()], want[1][free], want[3][free], torch.float32, "lse")
+
+
 # ------------------------------------------------------- value scales far apart
 @pytest.mark.parametrize("counts,page", [([2], 16), ([2], 64), ([100], 16), ([100], 128)])
 @pytest.mark.parametrize("order", [1, -1])
