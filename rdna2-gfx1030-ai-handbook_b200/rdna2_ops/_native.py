@@ -7,7 +7,6 @@ device is missing.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import os
@@ -147,11 +146,6 @@ def check(status, what):
     if status != 0:
         msg = library().b2_error_string(status)
         raise RuntimeError(f"{what} failed: {msg.decode() if msg else status}")
-
-
-def on_device(device):
-    """A context in which `device` is the current one."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def launch(device, name, *args):

@@ -53,8 +53,8 @@ def _rows(x):
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_bytes(device, *shape):
-    with nat.on_device(device):
+def _workspace_bytes(index, *shape):
+    with torch.cuda.device(index):
         return nat.library().b2_kv_attention_workspace_bytes(*shape)
 
 
@@ -211,7 +211,7 @@ class PagedKVCache:
         if tokens:
             q = _rows(q)
             stream = nat.stream_ptr(dev)
-            need = _workspace_bytes(dev, tokens, batch, max_new, heads, self.kv_heads, self.head_dim, width,
+            need = _workspace_bytes(dev.index, tokens, batch, max_new, heads, self.kv_heads, self.head_dim, width,
                                     self.page_size, window or 0)
             work = self._workspaces.get(stream)
             if work is None or work.numel() < need:

@@ -34,7 +34,7 @@ class Notes:
 
     @contextlib.contextmanager
     def device(self, device):
-        before, self.current = self.current, device.index
+        before, self.current = self.current, getattr(device, "index", device)
         yield
         self.current = before
 
