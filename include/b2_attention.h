@@ -70,7 +70,10 @@ int b2_kv_read(const void* k_codes, const void* v_codes, const float* k_scale, c
  * window > 0 only j > p - window.  out [tokens, q_heads, dim] in q's dtype
  * and, where lse is given, the natural logarithm of each row's sum of
  * exponentials [tokens, q_heads]; a row that sees nothing gives zeros and
- * -inf.  max_new bounds the tokens of one sequence.  The workspace holds
+ * -inf.  Scales are not negative, value scales below 2^-100 count as 2^-100,
+ * and e4m3 codes before a sequence's end are no NaN; a scale that is NaN or
+ * infinite makes NaN of the rows that see its block, and of no others.
+ * max_new bounds the tokens of one sequence.  The workspace holds
  * b2_kv_attention_workspace_bytes bytes, 256-byte aligned, zero-filled
  * before its first call; every call leaves it ready for the next one on the
  * same stream, of any shape that it is large enough for. */

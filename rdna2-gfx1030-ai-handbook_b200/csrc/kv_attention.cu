@@ -34,10 +34,10 @@
 // of 16-token stages, filled by TMA, and its own softmax; the warps of a CTA,
 // and the CTAs that share a (sequence, kv head), are joined at its end.
 //
-// Memory should bound it and does not quite: about 410 instructions a warp for
+// Memory should bound it and does not quite: about 420 instructions a warp for
 // 16 tokens of K and V, a third of them conversions.  One sequence of 262131
-// tokens, 8 kv heads of 128, 4 rows each, e4m3: 108 us for 537 MB, 5.0 TB/s;
-// 64 sequences of up to 8192, 8 rows each, int8: 120 us, 4.3 TB/s.
+// tokens, 8 kv heads of 128, 4 rows each, e4m3: 111 us for 537 MB, 4.8 TB/s;
+// 64 sequences of up to 8192, 8 rows each, int8: 123 us, 4.2 TB/s.
 #include "../../include/b2_attention.h"
 #include "b2_internal.h"
 #include "kv_attention.cuh"
@@ -687,9 +687,10 @@ cudaError_t run_rows_any(const AttendParams& p, int dim, int code, int nt, int g
 }
 
 // Most query rows of a (sequence, kv head) that kv_rows_kernel takes: what
-// one of its passes over the cache serves.  Measured for 24 rows, the two
-// kernels are level (8 heads over 32768 tokens 74 and 73 us, 16 sequences of
-// 4096 tokens 113 and 103 us), and from 32 rows on the tiles are ahead.
+// one of its passes over the cache serves.  Measured with this kernel and with
+// the tiles, 8 kv heads of 128 over 32768 tokens and 16 sequences of 4096:
+// 16 rows 72 and 78 us against 73 and 99, 24 rows 82 and 117 against 73 and 99,
+// 32 rows 84 and 119 against 69 and 96.
 constexpr int64_t kRowsMost = 16;
 
 // How a call is launched: on tensor-core tiles, or with `nt` times 8 columns

@@ -20,7 +20,7 @@ constexpr float kMostWeight = 49152.0f;
 // of it would be with a reference 2^5 above the largest.  What lies between
 // here and kMostWeight is what later tokens may bring before the reference is
 // raised, which the tile kernel pays for with a second pass over a tile: an
-// 8192-token prompt takes 698 us with 6, 690, 683 and 676 us with 3, 0 and -5.
+// 8192-token prompt takes 695 us with 6, 688, 680 and 677 us with 3, 0 and -5.
 constexpr float kReferenceLog2 = 6.0f;
 
 struct AttendParams {

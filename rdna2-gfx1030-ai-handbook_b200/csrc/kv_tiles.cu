@@ -20,9 +20,10 @@
 // A block of 128 rows or fewer uses row tile 0 alone.
 //
 // Measured: an 8192-token causal prompt, 32 query and 8 kv heads of 128, int8:
-// 660 us, 833 TFLOP/s.  A pair of row tiles x 128 tokens takes about 4400
-// cycles, 2048 of them of the tensor pipe and as many of the exponential unit:
-// the chain scores, weights, sums, next scores of a row tile bounds it.
+// 696 us, 790 TFLOP/s.  A pair of row tiles x 128 tokens takes about 5500
+// cycles, starts, ends and raised references included, 2048 of them of the
+// tensor pipe and as many of the exponential unit: the chain scores, weights,
+// sums, next scores of a row tile bounds it.
 //
 // The two row tiles alternate on the tensor cores: while one is in its
 // softmax the other multiplies, and they take turns so that it stays that way
@@ -824,8 +825,8 @@ cudaError_t launch_tiles(const TilesParams& tp, cudaStream_t stream) {
 template <int DIM, int CODE>
 cudaError_t launch_tiles_page(const TilesParams& tp, cudaStream_t stream) {
   if (tp.a.page_shift >= 6) return launch_tiles<DIM, CODE, 64>(tp, stream);
-  // pages of 32, an 8192-token prompt of 32 heads of 128: 662 us with their
-  // own variant, 750 us with that of 16; heads of 64: 565 and 536 us
+  // pages of 32, an 8192-token prompt of 32 heads of 128: 735 us with their
+  // own variant, 847 us with that of 16; heads of 64: 633 and 623 us
   if constexpr (DIM == 128) {
     if (tp.a.page_shift == 5) return launch_tiles<DIM, CODE, 32>(tp, stream);
   }

@@ -18,7 +18,14 @@ not read on the host: one lengths tensor serves every layer of a step.
 
 Tokens at negative positions, past the table, or on a table entry outside the
 cache (-1 marks an absent page) are not stored and not seen.  A page that a
-call appends to must belong to one sequence only.  Scales are not negative.
+call appends to must belong to one sequence only.
+
+What attend relies on where a cache holds other data than append wrote: scales
+are not negative, a value scale below 2**-100 counts as 2**-100 (append writes
+none, and zero goes with codes of zero), and e4m3 codes are no NaN, but behind
+the last token of a sequence.  A scale that is NaN or infinite shows in the rows
+that see its block, in all of their channels, and in no others.
+
 The workspace of attend is kept for each stream, so one cache may serve calls
 on several; ordering its appends before the calls that read them is the
 caller's, as for any tensor.
