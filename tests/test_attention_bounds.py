@@ -33,3 +33,19 @@ def test_a_window_over_everything(window, counts, causal):
         want = cache.attend(*args, offsets=off, causal=causal, max_new=min(most, sum(counts)), return_lse=True)
         got = cache.attend(*args, offsets=off, causal=causal, window=window, max_new=most, return_lse=True)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,page,dim", [([1, 1, 1], 16, 128), ([40, 1, 7], 16, 64), ([300, 130, 0], 64, 128)])
+def test_tables_far_wider_than_their_sequences(counts, page, dim):
+    """As wide as the longest context that a server allows: parts of the tile
+    kernel go by the width, and most of them find no tokens."""
+    from test_gpu_attention_exactness import _check, _queries
+    from test_gpu_kv_cache import _filled, _paging
+    lengths = [400, 31, 130]
+    narrow, pages = _paging(lengths, page, random.Random(4))
+    table = torch.full((3, 131072 // page), -1, dtype=torch.int32)
+    table[:, :narrow.shape[1]] = narrow
+    cache = _filled(pages, 2, dim, page, "int8", seed=9)
+    for kw in ({}, dict(window=90), dict(causal=False)):
+        _check(cache, _queries(counts, 8, dim), counts, lengths, table, **kw)
