@@ -106,8 +106,7 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 2^x by the exponential unit, within 2^-22 of itself; below 2^-126 zero.  The
-// library's exp2f adds a scaling for those, which no weight needs.
+// 2^x within 2^-22 of itself, and zero below 2^-126, which no weight needs.
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
